@@ -1,0 +1,370 @@
+// gpx_attend.hip -- host side of gpx_attend, gpx_attend_backward and gpx_attend_shared (include/gpx.h): checks, how the work is
+// cut, workspace layout, launches.  Kernels: gpx_attend_kernel.hpp (forward), gpx_attend_grad.hpp (gradients).
+//
+// Nothing is kept between calls and nothing is allocated: partial sums live in the caller's workspace.
+#include "gpx_attend.hpp"
+#include "gpx_model.hpp"
+
+namespace gpx {
+// 32, 64 or 128 packed rows per workgroup; what is left of its 4 waves takes parts of the key range.  (fp32 rows of more than 64
+// features: 64 at least, four waves' tiles of keys would not leave a wave its registers.)
+int attend_block_rows(bool f32, int dim, int rows) { return rows <= 32 && !(f32 && dim > 64) ? 32 : rows <= 64 ? 64 : 128; }
+int attend_block_keys(bool f32, int dim, int rows)
+{
+    const int bm = attend_block_rows(f32, dim, rows);
+    return f32 ? 128 * 32 / bm : bm == 128 ? 64 : 128;
+}
+int attend_dkv_block_rows(bool f32) { return f32 ? 32 : 64; }
+}  // namespace gpx
+
+namespace {
+
+struct DeviceScope {  // the call runs on args->device; the caller's current device is restored
+    int before = -1;
+    ~DeviceScope()
+    {
+        if (before >= 0)
+            (void)hipSetDevice(before);
+    }
+    int enter(int dev)
+    {
+        if (dev < 0)
+            return GPX_OK;
+        int cur = -1;
+        HIPCHK(hipGetDevice(&cur));
+        if (cur == dev)
+            return GPX_OK;
+        HIPCHK(hipSetDevice(dev));
+        before = cur;
+        return GPX_OK;
+    }
+};
+
+constexpr int64_t MOST_ROWS = (int64_t)1 << 30;  // row counts, and rows x heads of a call, stay in 32 bits
+
+int elem_size(const gpx_attend_args &a) { return a.scalar == GPX_F32 ? 4 : 2; }
+
+// strides keep every row of `dim` elements on a 16-byte boundary
+int check_view(const gpx_attend_args &a, const gpx_view &v, bool needed, const char *name)
+{
+    if (!needed)
+        return GPX_OK;
+    if (!v.p)
+        return fail(GPX_E_NULL, std::string("Empty data pointer: ") + name);
+    const int64_t m = 16 / elem_size(a);
+    if ((uintptr_t)v.p % 16 || v.batch % m || v.row % m || v.head % m)
+        return fail(GPX_E_BAD_ARG, std::string(name) + ": base and strides must be multiples of 16 bytes");
+    if (v.batch < 0 || v.row < 0 || v.head < 0)
+        return fail(GPX_E_BAD_ARG, std::string(name) + ": strides must not be negative");
+    return GPX_OK;
+}
+
+int check_args(const gpx_attend_args *pa, int which)
+{
+    if (!pa)
+        return fail(GPX_E_NULL, "Empty argument pointer");
+    const gpx_attend_args &a = *pa;
+    if (which != GPX_ATTEND_FORWARD && which != GPX_ATTEND_BACKWARD && which != GPX_ATTEND_SHARED)
+        return fail(GPX_E_BAD_ARG, "unknown attention call");
+    if (a.scalar != GPX_F32 && a.scalar != GPX_F16 && a.scalar != GPX_BF16)
+        return fail(GPX_E_BAD_ARG, "scalar must be GPX_F32, GPX_F16 or GPX_BF16");
+    if (a.heads < 1 || a.heads_kv < 1 || a.heads % a.heads_kv)
+        return fail(GPX_E_BAD_ARG, "heads must be a positive multiple of heads_kv");
+    if (a.dim < 8 || a.dim > ATTEND_MAX_DIM || a.dim % 8)
+        return fail(GPX_E_BAD_ARG, "dim must be a multiple of 8 up to 128");
+    if (a.batch < 0 || a.nq < 0 || a.nk < 0 || a.n_own < 0)
+        return fail(GPX_E_BAD_ARG, "negative size");
+    if (!(a.scale > 0.0) || !std::isfinite(a.scale) || !std::isfinite((float)(a.scale * ATTEND_LOG2E)))
+        return fail(GPX_E_BAD_ARG, "scale must be positive and finite");
+    if (a.batch > MOST_ROWS || a.nq > MOST_ROWS || a.nk > MOST_ROWS || a.n_own > MOST_ROWS || a.heads > 65536 ||
+        a.batch * a.nq > MOST_ROWS || a.batch * a.nq * a.heads > MOST_ROWS ||
+        (a.batch > 0 && (std::max(a.nk, a.n_own) / 32 + 1) * a.heads_kv > MOST_ROWS / a.batch))
+        return fail(GPX_E_BAD_ARG, "too many rows for one call");
+    return GPX_OK;
+}
+
+int check_data(const gpx_attend_args &a, int which)
+{
+    const bool rows = a.batch > 0 && a.nq > 0, keys = a.batch > 0 && a.nk > 0, own = a.batch > 0 && a.n_own > 0;
+    int rc;
+#define VIEW(V_, N_)                               \
+    if ((rc = check_view(a, a.V_, N_, #V_)) != GPX_OK) \
+    return rc
+    VIEW(q, rows);
+    VIEW(k, keys);
+    VIEW(v, keys);
+    VIEW(o, rows);
+    if (rows && !a.lse)
+        return fail(GPX_E_NULL, "Empty data pointer: lse");
+    if (which == GPX_ATTEND_SHARED) {
+        VIEW(k_own, own);
+        VIEW(v_own, own);
+    }
+    if (which == GPX_ATTEND_BACKWARD) {
+        VIEW(d_o, rows);
+        VIEW(dq, rows);
+        VIEW(dk, keys);
+        VIEW(dv, keys);
+    }
+#undef VIEW
+    return GPX_OK;
+}
+
+// `pieces` of [0, n) in whole steps of `step`: enough workgroups to give every CU two where `blocks` alone would not give it one
+void cut(int64_t blocks, int64_t n, int step, int least, int cus, int *pieces, int *chunk)
+{
+    int64_t p = 1;
+    if (blocks < cus && blocks > 0)
+        p = std::min<int64_t>((2 * cus + blocks - 1) / blocks, n / ((int64_t)step * least));
+    p = std::max<int64_t>(p, 1);
+    const int64_t steps = std::max<int64_t>(1, (n + step - 1) / step), per = (steps + p - 1) / p;
+    *chunk = (int)(per * step);
+    *pieces = (int)((steps + per - 1) / per);
+}
+
+int64_t blocks_of(int64_t rows, int64_t per) { return (rows + per - 1) / per; }
+
+struct Plan {
+    int splits = 1, chunk = 0;          // forward / the shared context
+    int own_splits = 0, own_chunk = 0;  // the own part
+    int k_splits = 1, k_chunk = 0;      // backward, dK dV: pieces of the rows
+    size_t ml = 0, po = 0, pk = 0, pv = 0, total = 0;  // offsets into the workspace (ml: the row statistics in a backward call)
+};
+
+size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+Plan plan_of(const gpx_attend_args &a, int which, int cus)
+{
+    Plan p;
+    const int64_t G = a.heads / a.heads_kv;
+    const bool f32 = a.scalar == GPX_F32;
+    const size_t rid = (size_t)a.batch * a.nq * a.heads;
+    if (which == GPX_ATTEND_SHARED) {
+        const int R = (int)(a.batch * a.nq * G), Ro = (int)(a.nq * G);
+        if (a.nk > 0)
+            cut(blocks_of(R, attend_block_rows(f32, (int)a.dim, R)) * a.heads_kv, a.nk, attend_block_keys(f32, (int)a.dim, R), 2, cus, &p.splits, &p.chunk);
+        else
+            p.splits = 0;
+        if (a.n_own > 0 || a.nk == 0)
+            cut(blocks_of(Ro, attend_block_rows(f32, (int)a.dim, Ro)) * a.heads_kv * a.batch, a.n_own, attend_block_keys(f32, (int)a.dim, Ro), 2, cus, &p.own_splits,
+                &p.own_chunk);
+        const size_t slots = p.splits + p.own_splits;
+        p.ml = 0;
+        p.po = up(slots * rid * sizeof(float2));
+        p.total = p.po + slots * rid * a.dim * sizeof(float);
+        return p;
+    }
+    const int R = (int)(a.nq * G);
+    const int64_t blocks = blocks_of(R, attend_block_rows(f32, (int)a.dim, R)) * a.heads_kv * a.batch;
+    if (which == GPX_ATTEND_FORWARD) {
+        cut(blocks, a.nk, attend_block_keys(f32, (int)a.dim, R), 2, cus, &p.splits, &p.chunk);
+        if (p.splits > 1) {
+            p.po = up(p.splits * rid * sizeof(float2));
+            p.total = p.po + p.splits * rid * a.dim * sizeof(float);
+        }
+        return p;
+    }
+    cut(blocks, a.nk, 32 * (128 / attend_block_rows(f32, (int)a.dim, R)), 2, cus, &p.splits, &p.chunk);
+    cut(blocks_of(a.nk, ATTEND_DKV_KEYS) * a.heads_kv * a.batch, R, attend_dkv_block_rows(f32), 2, cus, &p.k_splits, &p.k_chunk);
+    size_t at = up(rid * sizeof(float2));
+    p.po = at;
+    if (p.splits > 1)
+        at = up(at + p.splits * rid * a.dim * sizeof(float));
+    const size_t kv = (size_t)a.batch * a.nk * a.heads_kv * a.dim * sizeof(float);
+    p.pk = at;
+    if (p.k_splits > 1)
+        at = up(at + p.k_splits * kv);
+    p.pv = at;
+    if (p.k_splits > 1)
+        at = up(at + p.k_splits * kv);
+    p.total = at;
+    return p;
+}
+
+int cu_count(const gpx_attend_args &a)
+{
+    int dev = a.device;
+    if (dev < 0)
+        dev = device_backend()->get_device();
+    const int n = dev < 0 ? 0 : device_cu_count(dev);
+    return n > 0 ? n : 256;
+}
+
+AttendRows rows_of(const gpx_attend_args &a)
+{
+    AttendRows r;
+    r.q = a.q.p;
+    r.qb = a.q.batch, r.qr = a.q.row, r.qh = a.q.head;
+    r.len = a.q_len;
+    r.M = (int)a.nq;
+    r.G = (int)(a.heads / a.heads_kv);
+    r.Hk = (int)a.heads_kv;
+    r.D = (int)a.dim;
+    r.R = r.M * r.G;
+    r.grid_b = (int)a.batch;
+    return r;
+}
+AttendKeys keys_of(const gpx_view &k, const gpx_view &v, int64_t n, const int32_t *len, const uint8_t *mask, int64_t mask_b)
+{
+    AttendKeys s;
+    s.k = k.p, s.v = v.p;
+    s.kb = k.batch, s.kr = k.row, s.kh = k.head;
+    s.vb = v.batch, s.vr = v.row, s.vh = v.head;
+    s.n = (int)n;
+    s.len = len;
+    s.mask = mask;
+    s.mask_b = mask_b;
+    return s;
+}
+
+template <typename F>
+int by_type(const gpx_attend_args &a, F &&f)
+{
+    switch (a.scalar) {
+    case GPX_F32: f(float()); break;
+    case GPX_F16: f(_Float16()); break;
+    default: f(__bf16()); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+        return fail(GPX_E_HIP, hipGetErrorString(e));
+    return GPX_OK;
+}
+
+int begin(const gpx_attend_args *pa, int which, DeviceScope &scope, Plan *plan)
+{
+    int rc = check_args(pa, which);
+    if (rc == GPX_OK)
+        rc = check_data(*pa, which);
+    if (rc != GPX_OK)
+        return rc;
+    if (gpx_device_count() < 1)
+        return fail(GPX_E_NO_DEVICE, "no HIP device: libgpx has no CPU path");
+    rc = scope.enter(pa->device);
+    if (rc != GPX_OK)
+        return rc;
+    *plan = plan_of(*pa, which, cu_count(*pa));
+    if (plan->total > pa->workspace_bytes || (plan->total && (!pa->workspace || (uintptr_t)pa->workspace % 256)))
+        return fail(GPX_E_SIZE_MISMATCH, "workspace: gpx_attend_workspace bytes on a 256-byte boundary are needed");
+    return GPX_OK;
+}
+
+}  // namespace
+
+extern "C" int gpx_attend_workspace(const gpx_attend_args *args, int which, size_t *bytes)
+{
+    if (!bytes)
+        return fail(GPX_E_NULL, "Empty data pointer: bytes");
+    const int rc = check_args(args, which);
+    if (rc != GPX_OK)
+        return rc;
+    *bytes = plan_of(*args, which, cu_count(*args)).total;
+    return GPX_OK;
+}
+
+extern "C" int gpx_attend(const gpx_attend_args *args)
+{
+    DeviceScope scope;
+    Plan p;
+    const int rc = begin(args, GPX_ATTEND_FORWARD, scope, &p);
+    if (rc != GPX_OK)
+        return rc;
+    const gpx_attend_args &a = *args;
+    if (a.batch == 0 || a.nq == 0)
+        return GPX_OK;
+    AttendFwd f;
+    f.rows = rows_of(a);
+    f.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
+    f.c = (float)(a.scale * ATTEND_LOG2E);
+    f.splits = p.splits, f.chunk = p.chunk;
+    f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
+    f.lse = a.lse;
+    f.slot_rows = (long)(a.batch * a.nq * a.heads);
+    if (p.splits > 1) {
+        f.pml = (float2 *)((char *)a.workspace + p.ml);
+        f.po = (float *)((char *)a.workspace + p.po);
+    }
+    return by_type(a, [&](auto t) {
+        using T = decltype(t);
+        attend_launch_fwd<T>(f, (hipStream_t)a.stream);
+        if (p.splits > 1)
+            attend_launch_join<T>({f.po, f.pml, p.splits, f.slot_rows, (int)a.nq, (int)a.heads, (int)a.dim, f.o, f.ob, f.orow, f.oh, f.lse},
+                                  (hipStream_t)a.stream);
+    });
+}
+
+extern "C" int gpx_attend_shared(const gpx_attend_args *args)
+{
+    DeviceScope scope;
+    Plan p;
+    const int rc = begin(args, GPX_ATTEND_SHARED, scope, &p);
+    if (rc != GPX_OK)
+        return rc;
+    const gpx_attend_args &a = *args;
+    if (a.q_len || a.k_len || a.key_mask)
+        return fail(GPX_E_BAD_ARG, "gpx_attend_shared takes own_len only");
+    if (a.batch == 0 || a.nq == 0)
+        return GPX_OK;
+    AttendFwd f;
+    f.c = (float)(a.scale * ATTEND_LOG2E);
+    f.slot_rows = (long)(a.batch * a.nq * a.heads);
+    f.pml = (float2 *)((char *)a.workspace + p.ml);
+    f.po = (float *)((char *)a.workspace + p.po);
+    // the shared context: the rows of the whole batch are rows of one grid entry
+    AttendFwd s = f;
+    s.rows = rows_of(a);
+    s.rows.R = (int)(a.batch * a.nq) * s.rows.G;
+    s.rows.grid_b = 1;
+    s.keys = keys_of(a.k, a.v, a.nk, nullptr, nullptr, 0);
+    s.splits = p.splits, s.chunk = p.chunk;
+    // the own part
+    AttendFwd w = f;
+    w.rows = rows_of(a);
+    w.keys = keys_of(a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
+    w.tail = 1;
+    w.splits = p.own_splits, w.chunk = p.own_chunk;
+    w.slot0 = p.splits;
+    return by_type(a, [&](auto t) {
+        using T = decltype(t);
+        if (p.splits)
+            attend_launch_fwd<T>(s, (hipStream_t)a.stream);
+        if (p.own_splits)
+            attend_launch_fwd<T>(w, (hipStream_t)a.stream);
+        attend_launch_join<T>({f.po, f.pml, p.splits + p.own_splits, f.slot_rows, (int)a.nq, (int)a.heads, (int)a.dim, a.o.p, a.o.batch, a.o.row,
+                               a.o.head, a.lse},
+                              (hipStream_t)a.stream);
+    });
+}
+
+extern "C" int gpx_attend_backward(const gpx_attend_args *args)
+{
+    DeviceScope scope;
+    Plan p;
+    const int rc = begin(args, GPX_ATTEND_BACKWARD, scope, &p);
+    if (rc != GPX_OK)
+        return rc;
+    const gpx_attend_args &a = *args;
+    if (a.batch == 0)
+        return GPX_OK;
+    AttendBwd b;
+    b.rows = rows_of(a);
+    b.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
+    b.c = (float)(a.scale * ATTEND_LOG2E);
+    b.scale = (float)a.scale;
+    b.o = a.o.p, b.ob = a.o.batch, b.orow = a.o.row, b.oh = a.o.head;
+    b.dout = a.d_o.p, b.gb = a.d_o.batch, b.gr = a.d_o.row, b.gh = a.d_o.head;
+    b.lse = a.lse;
+    b.stat = (float2 *)((char *)a.workspace + p.ml);
+    b.dq = a.dq.p, b.dqb = a.dq.batch, b.dqr = a.dq.row, b.dqh = a.dq.head;
+    b.dk = a.dk.p, b.dkb = a.dk.batch, b.dkr = a.dk.row, b.dkh = a.dk.head;
+    b.dv = a.dv.p, b.dvb = a.dv.batch, b.dvr = a.dv.row, b.dvh = a.dv.head;
+    b.q_splits = p.splits, b.q_chunk = p.chunk;
+    b.k_splits = p.k_splits, b.k_chunk = p.k_chunk;
+    if (p.splits > 1)
+        b.pq = (float *)((char *)a.workspace + p.po);
+    if (p.k_splits > 1) {
+        b.pk = (float *)((char *)a.workspace + p.pk);
+        b.pv = (float *)((char *)a.workspace + p.pv);
+    }
+    return by_type(a, [&](auto t) { attend_launch_bwd<decltype(t)>(b, (hipStream_t)a.stream); });
+}

@@ -69,6 +69,7 @@ EXPORTS = [
     "gpx_model_prepare_variance", "gpx_model_get",
     "gpx_model_sync", "gpx_model_destroy", "gpx_model_create_shell", "gpx_model_state_blob", "gpx_model_commit",
     "gpx_model_replicate", "gpx_slab_range", "gpx_model_evaluate_sharded", "gpx_model_sample_surface_sharded", "gpx_trim", "gpx_debug_reload", "gpx_model_march_surface",
+    "gpx_attend", "gpx_attend_backward", "gpx_attend_shared", "gpx_attend_workspace",
     "gpx_dev_kbuild", "gpx_dev_kqp", "gpx_dev_kqp_f32", "gpx_padded_n", "gpx_dgp_create", "gpx_dgp_evaluate", "gpx_dgp_get",
     "gpx_dgp_add", "gpx_dgp_destroy", "gpx_dgp_loglik_gradient", "gpx_rprop_default", "gpx_dgp_optimise", "gpx_pcd_read", "gpx_node_training_set",
 ]

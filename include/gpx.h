@@ -349,6 +349,62 @@ typedef struct {
 void gpx_rprop_default(gpx_rprop *d);
 int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
 
+/* ---- softmax-weighted sums over a context (learned features; device arrays) ----------------------------------------------
+ * The counterpart of the mean f(q) = sum_j k(|q - p_j|) alpha_j (gp_regressor.hpp:332-357) for queries and points that carry
+ * learned feature vectors instead of three coordinates: per head  o_i = sum_j softmax_j(scale <q_i, k_j>) v_j  over the entries
+ * j of a context of another length, its gradients, and its form for a batch over one common context.  No reference equivalent.
+ *
+ * All data is on the device `device` (-1: the current one); calls are enqueued on `stream` (a hipStream_t, NULL: the default
+ * stream), never synchronise, allocate nothing and keep nothing, so they may be captured into a graph.  Two calls that can run
+ * at the same time (other streams, graphs replayed side by side) need workspaces of their own.
+ *
+ * A gpx_view is a tensor [batch][row][head][dim]: base pointer and element strides of the first three axes, dim contiguous;
+ * base and strides are multiples of 16 bytes, inputs may have zero strides, rows of an output must not overlap.  q, o, d_o, dq:
+ * [batch][nq][heads][dim]; k, v, dk, dv: [batch][nk][heads_kv][dim]; heads_kv divides heads, query head h reads key head
+ * h / (heads / heads_kv).  dim: a multiple of 8 up to 128.  lse: [batch][heads][nq] floats, contiguous: log sum_j exp(score).
+ *
+ * Which entries count: j < k_len[b] (int32 on the device; NULL: nk; values outside [0, nk] are clamped) and, with a mask,
+ * key_mask[b key_mask_batch + j] != 0.  What the others hold (NaN included) has no effect and their gradients are zero.
+ * Queries i >= q_len[b] (NULL: nq) do not count: their o and dq are zero, lse -inf, and they add nothing to dk, dv.  A
+ * query without any entry that counts has o = 0, lse = -inf and zero gradients.  Scores, sums and statistics are held in 32 bits;
+ * weights are rounded to the element type for the product with the values, outputs are rounded once.  Results do not depend on
+ * timing (fixed order of every sum, no atomics); they may differ in the last bits between devices of another size. */
+typedef enum { GPX_F32 = 0, GPX_F16 = 1, GPX_BF16 = 2 } gpx_scalar;
+typedef enum { GPX_ATTEND_FORWARD = 0, GPX_ATTEND_BACKWARD = 1, GPX_ATTEND_SHARED = 2 } gpx_attend_call;
+typedef struct {
+    void *p;
+    int64_t batch, row, head; /* elements */
+} gpx_view;
+typedef struct {
+    int32_t scalar; /* gpx_scalar of every view */
+    int32_t device;
+    int64_t batch, nq, nk, n_own;
+    int64_t heads, heads_kv, dim;
+    double scale; /* positive */
+    gpx_view q, k, v, o;
+    float *lse;
+    const int32_t *q_len, *k_len;
+    const uint8_t *key_mask;
+    int64_t key_mask_batch;
+    gpx_view d_o, dq, dk, dv; /* gpx_attend_backward */
+    gpx_view k_own, v_own;    /* gpx_attend_shared */
+    const int32_t *own_len;
+    void *workspace; /* 256-byte aligned, gpx_attend_workspace bytes; contents need no preparation */
+    size_t workspace_bytes;
+    void *stream;
+} gpx_attend_args;
+/* Bytes of workspace the call `which` needs for these sizes (0 is possible); reads no data. */
+int gpx_attend_workspace(const gpx_attend_args *args, int which, size_t *bytes);
+/* o and lse from q, k, v. */
+int gpx_attend(const gpx_attend_args *args);
+/* dq, dk, dv from d_o, q, k, v and the forward call's o and lse (same masks, lengths and scale). */
+int gpx_attend_backward(const gpx_attend_args *args);
+/* A batch over ONE context: k, v hold [nk][heads_kv][dim] (their batch stride is not used) and count for every query; k_own,
+ * v_own hold [batch][n_own][heads_kv][dim], of which own_len[b] entries exist (NULL: n_own) with the rows of the nq queries
+ * last: query i also sees the own entries j < own_len[b] - (nq - 1 - i).  One softmax over both.  The shared context is read
+ * once for the whole batch.  q_len, k_len and key_mask must be NULL. */
+int gpx_attend_shared(const gpx_attend_args *args);
+
 /* ---- stand-alone device stages (tests, bench roofline legs) -------------------------------
  * kbuild: K[i][j] = k(|p_i-p_j|) + sigma2_i*delta_ij on the lower block-triangle of an
  * n_padded x n_padded row-major matrix of `precision` scalars (identity on the padding);
