@@ -5,8 +5,8 @@ o_i = sum_j softmax_j(scale <q_i, k_j>) v_j.  Plumbing over the C ABI like gpx.p
 number comes from the HIP kernels, and there is no CPU fallback.
 
 Tensors are [batch, row, head, dim] of one type (float32, float16 or bfloat16) on one GPU; dim is a multiple of 8 up to 128 and the
-key heads divide the query heads.  Any strides will do as long as dim is contiguous and base and strides are multiples of 16
-bytes; other layouts are copied first.  Work is enqueued on the current stream of the tensors' device.  Gradients are explicit
+key heads divide the query heads.  Strided views are used as they are where gpx_view in include/gpx.h allows it (contiguous dim, base and
+strides multiples of 16 bytes); other layouts are copied first.  Work is enqueued on the current stream of the tensors' device.  Gradients are explicit
 calls, as for gpx_dgp_loglik_gradient: nothing here is recorded by autograd.
 """
 import ctypes as C
@@ -50,13 +50,13 @@ def _tensor(x, name, like=None, shape=None):
     return x
 
 
-def _usable(x):
-    """x itself, or a copy when the kernels cannot address it (include/gpx.h: contiguous dim, multiples of 16 bytes)."""
+def _usable(x, group=1):
+    """x itself, or a copy when the kernels cannot address it (gpx_view in include/gpx.h)."""
     if x.numel() == 0:
         return x
     m = 16 // x.element_size()
     b, r, h, d = x.stride()
-    if (d != 1 and x.shape[3] != 1) or b % m or r % m or h % m or x.data_ptr() % 16:
+    if d != 1 or b % m or r % m or h % m or x.data_ptr() % 16 or (r < x.shape[3] and x.shape[1] > 1) or r > 1 << 22 or h * group > 1 << 27:
         # clone: .contiguous() would hand back an offset view that is contiguous but not aligned
         return x.clone(memory_format=torch.contiguous_format)
     return x
@@ -128,7 +128,7 @@ def attend(q, k, v, scale=None, k_len=None, key_mask=None, q_len=None):
     _tensor(v, "v", q, (b, nk, hk, d))
     lens = (_lengths(q_len, "q_len", b, q.device), _lengths(k_len, "k_len", b, q.device))
     mask = _mask(key_mask, b, nk, q.device)
-    q, k, v = _usable(q), _usable(k), _usable(v)
+    q, k, v = _usable(q, hq // hk), _usable(k), _usable(v)
     o = torch.empty((b, nq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, hq, nq), dtype=torch.float32, device=q.device)
     _run(FORWARD, q, (b, nq, nk, 0, hq, hk, d), scale, _view(q) + _view(k) + _view(v) + _view(o), lse.data_ptr(), lens, mask,
@@ -151,7 +151,7 @@ def attend_backward(d_o, q, k, v, o, lse, scale=None, k_len=None, key_mask=None,
         _bad("lse must be of shape %s, not %s" % ([b, hq, nq], list(lse.shape)), E_SIZE_MISMATCH)
     lens = (_lengths(q_len, "q_len", b, q.device), _lengths(k_len, "k_len", b, q.device))
     mask = _mask(key_mask, b, nk, q.device)
-    q, k, v, o, d_o = _usable(q), _usable(k), _usable(v), _usable(o), _usable(d_o)
+    q, k, v, o, d_o = _usable(q, hq // hk), _usable(k), _usable(v), _usable(o), _usable(d_o, hq // hk)
     dq = torch.empty((b, nq, hq, d), dtype=q.dtype, device=q.device)
     dk = torch.empty((b, nk, hk, d), dtype=q.dtype, device=q.device)
     dv = torch.empty((b, nk, hk, d), dtype=q.dtype, device=q.device)
@@ -176,7 +176,7 @@ def attend_shared(q, k, v, k_own, v_own, own_len=None, scale=None):
     _tensor(k_own, "k_own", q, (b, no, hk, d))
     _tensor(v_own, "v_own", q, (b, no, hk, d))
     own = _lengths(own_len, "own_len", b, q.device)
-    q, k, v, k_own, v_own = _usable(q), _usable(k), _usable(v), _usable(k_own), _usable(v_own)
+    q, k, v, k_own, v_own = _usable(q, hq // hk), _usable(k), _usable(v), _usable(k_own), _usable(v_own)
     o = torch.empty((b, nq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, hq, nq), dtype=torch.float32, device=q.device)
     _run(SHARED, q, (b, nq, nk, no, hq, hk, d), scale, _view(q) + _view(k) + _view(v) + _view(o), lse.data_ptr(), (0, 0), (0, 0),

@@ -12,7 +12,7 @@ int attend_block_rows(bool f32, int dim, int rows) { return rows <= 32 && !(f32 
 int attend_block_keys(bool f32, int dim, int rows)
 {
     const int bm = attend_block_rows(f32, dim, rows);
-    return f32 ? 128 * 32 / bm : bm == 128 ? 64 : 128;
+    return f32 ? 128 * 32 / bm : bm == 32 ? 128 : 64;
 }
 int attend_dkv_block_rows(bool f32) { return f32 ? 32 : 64; }
 }  // namespace gpx
@@ -45,7 +45,8 @@ constexpr int64_t MOST_ROWS = (int64_t)1 << 30;  // row counts, and rows x heads
 int elem_size(const gpx_attend_args &a) { return a.scalar == GPX_F32 ? 4 : 2; }
 
 // strides keep every row of `dim` elements on a 16-byte boundary
-int check_view(const gpx_attend_args &a, const gpx_view &v, bool needed, const char *name)
+constexpr int64_t LONGEST_ROW = (int64_t)1 << 22, LONGEST_GROUP = (int64_t)1 << 27;
+int check_view(const gpx_attend_args &a, const gpx_view &v, bool needed, int64_t n_rows, int64_t group, const char *name)
 {
     if (!needed)
         return GPX_OK;
@@ -56,6 +57,11 @@ int check_view(const gpx_attend_args &a, const gpx_view &v, bool needed, const c
         return fail(GPX_E_BAD_ARG, std::string(name) + ": base and strides must be multiples of 16 bytes");
     if (v.batch < 0 || v.row < 0 || v.head < 0)
         return fail(GPX_E_BAD_ARG, std::string(name) + ": strides must not be negative");
+    // the kernels address one tile of rows (at most 128, and the heads of a group) with 32-bit byte offsets
+    if (v.row > LONGEST_ROW || (n_rows > 1 && v.row < a.dim))
+        return fail(GPX_E_BAD_ARG, std::string(name) + ": row stride below dim or above 2^22");
+    if (v.head > LONGEST_GROUP / std::max<int64_t>(1, group))
+        return fail(GPX_E_BAD_ARG, std::string(name) + ": the heads of a group must lie within 2^27 elements");
     return GPX_OK;
 }
 
@@ -87,24 +93,25 @@ int check_data(const gpx_attend_args &a, int which)
 {
     const bool rows = a.batch > 0 && a.nq > 0, keys = a.batch > 0 && a.nk > 0, own = a.batch > 0 && a.n_own > 0;
     int rc;
-#define VIEW(V_, N_)                               \
-    if ((rc = check_view(a, a.V_, N_, #V_)) != GPX_OK) \
+    const int64_t G = a.heads / a.heads_kv;
+#define VIEW(V_, ON_, N_, G_)                                 \
+    if ((rc = check_view(a, a.V_, ON_, N_, G_, #V_)) != GPX_OK) \
     return rc
-    VIEW(q, rows);
-    VIEW(k, keys);
-    VIEW(v, keys);
-    VIEW(o, rows);
+    VIEW(q, rows, a.nq, G);
+    VIEW(k, keys, a.nk, 1);
+    VIEW(v, keys, a.nk, 1);
+    VIEW(o, rows, a.nq, 1);
     if (rows && !a.lse)
         return fail(GPX_E_NULL, "Empty data pointer: lse");
     if (which == GPX_ATTEND_SHARED) {
-        VIEW(k_own, own);
-        VIEW(v_own, own);
+        VIEW(k_own, own, a.n_own, 1);
+        VIEW(v_own, own, a.n_own, 1);
     }
     if (which == GPX_ATTEND_BACKWARD) {
-        VIEW(d_o, rows);
-        VIEW(dq, rows);
-        VIEW(dk, keys);
-        VIEW(dv, keys);
+        VIEW(d_o, rows, a.nq, G);
+        VIEW(dq, rows, a.nq, 1);
+        VIEW(dk, keys, a.nk, 1);
+        VIEW(dv, keys, a.nk, 1);
     }
 #undef VIEW
     return GPX_OK;
@@ -354,7 +361,8 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.o = a.o.p, b.ob = a.o.batch, b.orow = a.o.row, b.oh = a.o.head;
     b.dout = a.d_o.p, b.gb = a.d_o.batch, b.gr = a.d_o.row, b.gh = a.d_o.head;
     b.lse = a.lse;
-    b.stat = (float2 *)((char *)a.workspace + p.ml);
+    b.stat = (float *)((char *)a.workspace + p.ml);
+    b.div_g = DivBy((unsigned)b.rows.G);
     b.dq = a.dq.p, b.dqb = a.dq.batch, b.dqr = a.dq.row, b.dqh = a.dq.head;
     b.dk = a.dk.p, b.dkb = a.dk.batch, b.dkr = a.dk.row, b.dkh = a.dk.head;
     b.dv = a.dv.p, b.dvb = a.dv.batch, b.dvr = a.dv.row, b.dvh = a.dv.head;

@@ -56,6 +56,20 @@ struct AttendJoin {
     float *lse = nullptr;
 };
 
+// n / d for 0 <= n < 2^31 by a product (d >= 1): with 2^s >= d and f = floor(2^32 (2^s - d) / d) + 1 the quotient is
+// floor((n + floor(n f / 2^32)) / 2^s)
+struct DivBy {
+    unsigned f = 1, s = 0;
+    DivBy() = default;
+    explicit DivBy(unsigned d)
+    {
+        while ((1u << s) < d)
+            ++s;
+        f = (unsigned)((((unsigned long long)1 << 32) * (((unsigned long long)1 << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((unsigned)n, f) + (unsigned)n) >> s); }
+};
+
 struct AttendBwd {
     AttendRows rows;
     AttendKeys keys;
@@ -63,7 +77,8 @@ struct AttendBwd {
     const void *o = nullptr, *dout = nullptr;
     long ob = 0, orow = 0, oh = 0, gb = 0, gr = 0, gh = 0;
     const float *lse = nullptr;
-    float2 *stat = nullptr;  // [B][H][M]: lse in log2 units (+inf where the row has no weights), <dO, O>
+    float *stat = nullptr;   // [2][B][H][M]: lse in log2 units (+inf where the row has no weights); <dO, O>
+    DivBy div_g;             // by rows.G
     void *dq = nullptr, *dk = nullptr, *dv = nullptr;
     long dqb = 0, dqr = 0, dqh = 0, dkb = 0, dkr = 0, dkh = 0, dvb = 0, dvr = 0, dvh = 0;
     int q_splits = 1, q_chunk = 0;   // dQ: pieces of the key range

@@ -38,29 +38,34 @@ __global__ __launch_bounds__(256) void attend_stat_kernel(AttendBwd a, long rows
     if (on && sub == 0) {
         const float lse = valid ? a.lse[rid] : NEG_INF;
         const bool none = lse == NEG_INF;
-        a.stat[rid] = make_float2(none ? POS_INF : lse * 1.44269504088896f, none ? 0.0f : s);
+        a.stat[rid] = none ? POS_INF : lse * 1.44269504088896f;
+        a.stat[rows + rid] = none ? 0.0f : s;
     }
 }
 
-// dQ: waves as in the forward kernel.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
+// dQ: waves and tiles as in the forward kernel.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
 template <typename T, int DT, int WM>
 struct DqShape {
     static constexpr int WK = 4 / WM;
     static constexpr int KT = 32;
     static constexpr int BN = KT * WK;
     static constexpr int BM = 32 * WM;
+    static constexpr int LDS = 4 * BN * Tile<T, DT>::ROWB;
+    static constexpr int PER_CU = LDS <= 80 * 1024 - 1024 && (sizeof(T) == 2 || DT <= 2) ? 2 : 1;
 };
 
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 1)) void attend_dq_kernel(AttendBwd a)
+__global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_kernel(AttendBwd a)
 {
     using TL = Tile<T, DT>;
     using SH = DqShape<T, DT, WM>;
     constexpr int BN = SH::BN, WK = SH::WK, KT = SH::KT;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BN * TL::ROWB < 512 ? 512 : 2 * BN * TL::ROWB];
-    char *kt = lds, *vt = lds + BN * TL::ROWB;
+    using FL = Fill<T, DT, BN>;
+    constexpr int TILE_B = BN * TL::ROWB;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];
+    __shared__ __attribute__((aligned(16))) float bias[2][BN];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
     const int mtiles = (rw.R + SH::BM - 1) / SH::BM;
@@ -75,12 +80,61 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
     const int len = clamped(a.keys.len, bz, a.keys.n);
     const int begin = split * a.q_chunk, end = min(len, begin + a.q_chunk);
 
+    const unsigned ksb = (unsigned)(a.keys.kr * sizeof(T)), vsb = (unsigned)(a.keys.vr * sizeof(T));
+    const char *kp = (const char *)((const T *)a.keys.k + bz * a.keys.kb + hk * a.keys.kh);
+    const char *vp = (const char *)((const T *)a.keys.v + bz * a.keys.vb + hk * a.keys.vh);
+    const unsigned char *mask = a.keys.mask ? a.keys.mask + bz * a.keys.mask_b : nullptr;
+    const unsigned lds0 = lds_offset(lds);
+
+    unsigned ko[FL::N], vo[FL::N];
+#pragma unroll
+    for (int x = 0; x < FL::N; ++x) {
+        const unsigned c = FL::chunk(x, wave, lane, rw.D), r = FL::row(x, wave, lane);
+        ko[x] = c == DMA_OUT ? DMA_OUT : r * ksb + c;
+        vo[x] = c == DMA_OUT ? DMA_OUT : r * vsb + c;
+    }
+    unsigned mb[FL::N + 1];
+    const auto look = [&](int n0) {
+        if (!mask)
+            return;
+#pragma unroll
+        for (int x = 0; x < FL::N; ++x) {
+            const int j = n0 + FL::row(x, wave, lane);
+            mb[x] = j < end ? mask[j] : 0;
+        }
+        const int j = n0 + tid;
+        mb[FL::N] = tid < BN && j < end ? mask[j] : 0;
+    };
+    const auto fetch = [&](int n0, int stage) {
+        const unsigned left = (unsigned)(end - n0);
+        const u32x4 kd = dma_buffer(kp + (long)n0 * ksb, (unsigned)min((unsigned long long)left * ksb, (unsigned long long)DMA_MOST));
+        const u32x4 vd = dma_buffer(vp + (long)n0 * vsb, (unsigned)min((unsigned long long)left * vsb, (unsigned long long)DMA_MOST));
+        const unsigned at0 = lds0 + stage * 2 * TILE_B;
+#pragma unroll
+        for (int x = 0; x < FL::N; ++x)
+            if (FL::on(x, wave)) {
+                const bool off = mask && !mb[x];
+                dma16(kd, off ? DMA_OUT : ko[x], at0 + FL::lds(x, wave));
+                dma16(vd, off ? DMA_OUT : vo[x], at0 + TILE_B + FL::lds(x, wave));
+            }
+        if (tid < BN && (mask || n0 + BN > end))
+            bias[stage][tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
+    };
+    if (begin < end) {
+        look(begin);
+        fetch(begin, 0);
+        look(begin + BN);
+    }
+
     x8<T> qf[2 * DT], gf[2 * DT];
     load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
     load_row_frags<T, DT>(gf, (const T *)a.dout + (at.valid ? at.b * a.gb + at.i * a.gr + at.h * a.gh : 0), at.valid, rw.D, lane);
-    float2 stat = make_float2(POS_INF, 0.0f);
-    if (at.valid)
-        stat = a.stat[((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i];
+    float lse = POS_INF, dd = 0.0f;
+    if (at.valid) {
+        const long rid = ((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i;
+        lse = a.stat[rid];
+        dd = a.stat[(long)rw.grid_b * rw.Hk * rw.G * rw.M + rid];
+    }
 
     f32x16 dq[DT];
 #pragma unroll
@@ -89,34 +143,33 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
         for (int i = 0; i < 16; ++i)
             dq[d][i] = 0.0f;
 
-    const T *kp = (const T *)a.keys.k + bz * a.keys.kb + hk * a.keys.kh;
-    const T *vp = (const T *)a.keys.v + bz * a.keys.vb + hk * a.keys.vh;
-    const unsigned char *mask = a.keys.mask ? a.keys.mask + bz * a.keys.mask_b : nullptr;
-    const auto counts = [mask](int j) { return !mask || mask[j]; };
-    const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
-
-    Stage<T, DT, BN, 256> sk, sv;
-    if (begin < end) {
-        sk.load(kp, a.keys.kr, begin, end, rw.D, tid, counts);
-        sv.load(vp, a.keys.vr, begin, end, rw.D, tid, counts);
-    }
-    for (int n0 = begin; n0 < end; n0 += BN) {
-        const int j = n0 + wk * KT + (lane & 31);
-        const unsigned seen = (unsigned)__ballot(j < end && counts(j));
-        __syncthreads();
-        sk.store(kt, tid);
-        sv.store(vt, tid);
+    int stage = 0;
+    for (int n0 = begin; n0 < end; n0 += BN, stage ^= 1) {
+        dma_wait();
         __syncthreads();
         if (n0 + BN < end) {
-            sk.load(kp, a.keys.kr, n0 + BN, end, rw.D, tid, counts);
-            sv.load(vp, a.keys.vr, n0 + BN, end, rw.D, tid, counts);
+            fetch(n0 + BN, stage ^ 1);
+            look(n0 + 2 * BN);
         }
-        if (seen == 0)
-            continue;
+        const char *kt = lds + stage * 2 * TILE_B, *vt = kt + TILE_B;
+        const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
         f32x16 sc, dp;
+        if (mask || n0 + BN > end) {  // -inf where the key does not count: its weight, and with it dS, is zero
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage][wk * KT + 8 * x + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    sc[4 * x + j] = w[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                sc[i] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            sc[i] = dp[i] = 0.0f;
+            dp[i] = 0.0f;
 #pragma unroll
         for (int t = 0; t < TL::KS; ++t) {
             sc = mma(TL::row_frag(kt, rbase, wk * KT, t), qf[t], sc);
@@ -124,12 +177,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            sc[i] = exp2_(sc[i] * a.c - stat.x) * (dp[i] - stat.y);
-        if (seen != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                sc[i] = bit_of(seen, half, i) ? sc[i] : 0.0f;
-        }
+            sc[i] = exp2_(sc[i] * a.c - lse) * (dp[i] - dd);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const x8<T> ds = as_operand<T>(sc, t);
@@ -140,7 +188,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
     }
     if constexpr (WK > 1) {
         constexpr int PIECE = 64 * 16 * DT;
-        static_assert((WK - 1) * WM * PIECE * 4 <= 2 * BN * TL::ROWB, "the join uses the tiles' memory");
+        static_assert((WK - 1) * WM * PIECE * 4 <= 4 * TILE_B, "the join uses the tiles' memory");
         float *pc = reinterpret_cast<float *>(lds);
         __syncthreads();
         if (wk > 0) {
@@ -197,16 +245,28 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
 // dK, dV: 4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one
 // key, then dV^T += dO^T P and dK^T += Q^T dS.
 template <typename T, int DT>
-__global__ __launch_bounds__(256, 1) void attend_dkv_kernel(AttendBwd a)
+struct DkvShape {
+    static constexpr int BR = sizeof(T) == 2 ? 64 : 32;
+    static constexpr int PER_CU = sizeof(T) == 2 || DT <= 2 ? 2 : 1;
+};
+
+template <typename T, int DT>
+__global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_kernel(AttendBwd a)
 {
     using TL = Tile<T, DT>;
-    constexpr int BR = sizeof(T) == 2 ? 64 : 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BR * TL::ROWB];
-    __shared__ __attribute__((aligned(16))) float st_lse[BR];
-    __shared__ __attribute__((aligned(16))) float st_d[BR];
-    char *qt = lds, *gt = lds + BR * TL::ROWB;
+    constexpr int BR = DkvShape<T, DT>::BR;
+    using FL = Fill<T, DT, BR>;
+    constexpr int TILE_B = BR * TL::ROWB;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];      // [stage][Q, dO]
+    __shared__ __attribute__((aligned(1024))) float stat[2][2][64];      // [stage][lse, <dO, O>][row]
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    // 128 features fill the registers: what follows from the lane's number is formed again where it is needed, not kept
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto lane_again = [] {
+        int x = threadIdx.x & 63;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     const AttendRows &rw = a.rows;
     const int ktiles = (a.keys.n + ATTEND_DKV_KEYS - 1) / ATTEND_DKV_KEYS;
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
@@ -217,14 +277,50 @@ __global__ __launch_bounds__(256, 1) void attend_dkv_kernel(AttendBwd a)
     const int hk = id % rw.Hk, bz = id / rw.Hk;
 
     const int len = clamped(a.keys.len, bz, a.keys.n);
-    const int key = ktile * ATTEND_DKV_KEYS + wave * 32 + (lane & 31);
-    const bool exists = key < a.keys.n;
-    const bool counts = key < len && (!a.keys.mask || a.keys.mask[bz * a.keys.mask_b + key]);
-    const int begin = split * a.k_chunk, end = min(rw.R, begin + a.k_chunk);
+    const auto counts_of = [&](int key) { return key < len && (!a.keys.mask || a.keys.mask[bz * a.keys.mask_b + key]); };
+    const int key0 = ktile * ATTEND_DKV_KEYS + wave * 32;
+    // rows are packed (query, head of the group); queries from q_len on do not count
+    const int begin = split * a.k_chunk;
+    const int end = ktile * ATTEND_DKV_KEYS < len ? min(clamped(rw.len, bz, rw.M) * rw.G, begin + a.k_chunk) : 0;
+
+    const unsigned lds0 = lds_offset(lds), stat0 = lds_offset(stat);
+    const int h0 = hk * rw.G;
+    const T *qp = (const T *)rw.q + bz * rw.qb + h0 * rw.qh, *gp = (const T *)a.dout + bz * a.gb + h0 * a.gh;
+    const float *sp = a.stat + ((long)bz * rw.Hk * rw.G + h0) * rw.M;
+    const long stats = (long)rw.grid_b * rw.Hk * rw.G * rw.M;
+    const unsigned qrb = (unsigned)(rw.qr * sizeof(T)), qhb = (unsigned)(rw.qh * sizeof(T));
+    const unsigned grb = (unsigned)(a.gr * sizeof(T)), ghb = (unsigned)(a.gh * sizeof(T));
+    const auto fetch = [&](int r0, int stage) {
+        const int n0 = a.div_g(r0), lane = lane_again();
+        const u32x4 qd = dma_buffer(qp + (long)n0 * rw.qr, DMA_MOST), gd = dma_buffer(gp + (long)n0 * a.gr, DMA_MOST);
+        const unsigned at0 = lds0 + stage * 2 * TILE_B;
+#pragma unroll(DT > 2 ? 1 : FL::N)
+        for (int x = 0; x < FL::N; ++x)
+            if (FL::on(x, wave)) {
+                const int r = r0 + FL::row(x, wave, lane);
+                const int n = a.div_g(r), g = r - n * rw.G;
+                const unsigned c = FL::chunk(x, wave, lane, rw.D);
+                const bool off = r >= end || c == DMA_OUT;
+                dma16(qd, off ? DMA_OUT : (unsigned)(n - n0) * qrb + g * qhb + c, at0 + FL::lds(x, wave));
+                dma16(gd, off ? DMA_OUT : (unsigned)(n - n0) * grb + g * ghb + c, at0 + TILE_B + FL::lds(x, wave));
+            }
+        if (wave < 2) {  // a row past the end gets zeros, and has zeros for Q and dO: it adds nothing
+            const int r = r0 + lane;
+            const int n = a.div_g(r), g = r - n * rw.G;
+            const u32x4 sd = dma_buffer(sp + wave * stats + n0, DMA_MOST);
+            dma4(sd, lane < BR && r < end ? 4u * (g * rw.M + (n - n0)) : DMA_OUT, stat0 + (stage * 2 + wave) * 256);
+        }
+    };
+    if (begin < end)
+        fetch(begin, 0);
 
     x8<T> kf[2 * DT], vf[2 * DT];
-    load_row_frags<T, DT>(kf, (const T *)a.keys.k + bz * a.keys.kb + hk * a.keys.kh + (counts ? key * a.keys.kr : 0), counts, rw.D, lane);
-    load_row_frags<T, DT>(vf, (const T *)a.keys.v + bz * a.keys.vb + hk * a.keys.vh + (counts ? key * a.keys.vr : 0), counts, rw.D, lane);
+    {
+        const int lane = lane_again(), key = key0 + (lane & 31);
+        const bool counts = counts_of(key);
+        load_row_frags<T, DT>(kf, (const T *)a.keys.k + bz * a.keys.kb + hk * a.keys.kh + (counts ? key * a.keys.kr : 0), counts, rw.D, lane);
+        load_row_frags<T, DT>(vf, (const T *)a.keys.v + bz * a.keys.vb + hk * a.keys.vh + (counts ? key * a.keys.vr : 0), counts, rw.D, lane);
+    }
 
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -233,67 +329,30 @@ __global__ __launch_bounds__(256, 1) void attend_dkv_kernel(AttendBwd a)
         for (int i = 0; i < 16; ++i)
             dk[d][i] = dv[d][i] = 0.0f;
 
-    const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
-    constexpr int N = (BR * TL::NCH + 255) / 256;
-    u32x4 rq[N], rg[N];
-    float2 rs;
-    const auto load = [&](int r0) {
-#pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int cid = tid + x * 256, row = cid / TL::NCH, c = cid - row * TL::NCH;
-            u32x4 zq = {0, 0, 0, 0}, zg = {0, 0, 0, 0};
-            if ((BR * TL::NCH % 256 == 0 || row < BR) && r0 + row < end && c * TL::EPC < rw.D) {
-                const RowAt w = row_at(rw, bz, hk, r0 + row);
-                if (w.valid) {
-                    zq = *reinterpret_cast<const u32x4 *>((const T *)rw.q + w.b * rw.qb + w.i * rw.qr + w.h * rw.qh + c * TL::EPC);
-                    zg = *reinterpret_cast<const u32x4 *>((const T *)a.dout + w.b * a.gb + w.i * a.gr + w.h * a.gh + c * TL::EPC);
-                }
-            }
-            rq[x] = zq;
-            rg[x] = zg;
-        }
-        rs = make_float2(POS_INF, 0.0f);
-        if (tid < BR && r0 + tid < end) {
-            const RowAt w = row_at(rw, bz, hk, r0 + tid);
-            if (w.valid)
-                rs = a.stat[((long)w.b * rw.Hk * rw.G + w.h) * rw.M + w.i];
-        }
-    };
-    const bool work = ktile * ATTEND_DKV_KEYS < len;  // else nothing here counts: zeros
-    if (work && begin < end)
-        load(begin);
-    for (int r0 = begin; work && r0 < end; r0 += BR) {
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int cid = tid + x * 256, row = cid / TL::NCH, c = cid - row * TL::NCH;
-            if (BR * TL::NCH % 256 == 0 || row < BR) {
-                *reinterpret_cast<u32x4 *>(qt + TL::place(row, c)) = rq[x];
-                *reinterpret_cast<u32x4 *>(gt + TL::place(row, c)) = rg[x];
-            }
-        }
-        if (tid < BR) {
-            st_lse[tid] = rs.x;
-            st_d[tid] = rs.y;
-        }
+    int stage = 0;
+    for (int r0 = begin; r0 < end; r0 += BR, stage ^= 1) {
+        dma_wait();
         __syncthreads();
         if (r0 + BR < end)
-            load(r0 + BR);
-#pragma unroll
+            fetch(r0 + BR, stage ^ 1);
+#pragma unroll 1
         for (int s = 0; s < BR / 32; ++s) {
+            const int lane = lane_again(), half = lane >> 5, at0 = stage * 2 * TILE_B + s * 32 * TL::ROWB;
+            const int rbase = TL::row_base(lane) + at0, cbase = TL::col_base(lane) + at0;
+            const char *qt = lds, *gt = lds + TILE_B;
             f32x16 p, dp;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 p[i] = dp[i] = 0.0f;
 #pragma unroll
             for (int t = 0; t < TL::KS; ++t) {
-                p = mma(TL::row_frag(qt, rbase, 32 * s, t), kf[t], p);
-                dp = mma(TL::row_frag(gt, rbase, 32 * s, t), vf[t], dp);
+                p = mma(TL::row_frag(qt, rbase, 0, t), kf[t], p);
+                dp = mma(TL::row_frag(gt, rbase, 0, t), vf[t], dp);
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const f32x4 ls = *reinterpret_cast<const f32x4 *>(st_lse + 32 * s + 8 * x + 4 * half);
-                const f32x4 ds = *reinterpret_cast<const f32x4 *>(st_d + 32 * s + 8 * x + 4 * half);
+                const f32x4 ls = *reinterpret_cast<const f32x4 *>(&stat[stage][0][32 * s + 8 * x + 4 * half]);
+                const f32x4 ds = *reinterpret_cast<const f32x4 *>(&stat[stage][1][32 * s + 8 * x + 4 * half]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int i = 4 * x + j;
@@ -303,17 +362,24 @@ __global__ __launch_bounds__(256, 1) void attend_dkv_kernel(AttendBwd a)
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const x8<T> w = as_operand<T>(p, t), ws = as_operand<T>(dp, t);
+                const x8<T> w = as_operand<T>(p, t);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    dv[d] = mma(TL::col_frag(gt, cbase, 32 * s + 16 * t, d), w, dv[d]);
-                    dk[d] = mma(TL::col_frag(qt, cbase, 32 * s + 16 * t, d), ws, dk[d]);
-                }
+                for (int d = 0; d < DT; ++d)
+                    dv[d] = mma(TL::col_frag(gt, cbase, 16 * t, d), w, dv[d]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const x8<T> w = as_operand<T>(dp, t);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    dk[d] = mma(TL::col_frag(qt, cbase, 16 * t, d), w, dk[d]);
             }
         }
     }
-    if (!exists)
+    const int lane = lane_again(), half = lane >> 5, key = key0 + (lane & 31);
+    if (key >= a.keys.n)
         return;
+    const bool counts = counts_of(key);
     // a key that does not count had zeros for its fragments: its sums are of finite weights but not zero
     const float fk = counts ? 1.0f : 0.0f;
     if (a.pk) {

@@ -10,25 +10,31 @@ namespace attend {
 // One workgroup of 4 waves: WM waves along the rows (32 packed rows each), WK = 4 / WM along the keys.  Scores are formed
 // TRANSPOSED, S^T = K Q^T: a lane then holds one row's weights (its column), the running maximum and sum of a row are one
 // register per lane, and S^T turns into the operand of O^T = V^T P^T without leaving the lane (gpx_attend_tile.hpp).
-// Keys and values are read from memory once per 32 WM rows, as tiles of BN rows through LDS.
+// Keys and values are read from memory once per 32 WM rows, as tiles of BN rows, two of them in LDS: while one is worked on the
+// next is on its way.
 template <typename T, int DT, int WM>
 struct FwdShape {
     static constexpr int WK = 4 / WM;
-    static constexpr int KT = sizeof(T) == 2 && WK < 4 ? 64 : 32;  // keys of a wave per step
+    static constexpr int KT = sizeof(T) == 2 && WK == 1 ? 64 : 32;  // keys of a wave per step
     static constexpr int BN = KT * WK;
     static constexpr int BM = 32 * WM;
+    static constexpr int LDS = 4 * BN * Tile<T, DT>::ROWB;
+    // workgroups a CU has room for (its 160 KB of LDS, and two waves per SIMD where the registers allow it)
+    static constexpr int PER_CU = LDS <= 80 * 1024 - 1024 ? 2 : 1;
 };
 
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 1)) void attend_fwd_kernel(AttendFwd a)
+__global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd_kernel(AttendFwd a)
 {
     using TL = Tile<T, DT>;
     using SH = FwdShape<T, DT, WM>;
     constexpr int BN = SH::BN, WK = SH::WK, KT = SH::KT, NS = KT / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BN * TL::ROWB];
-    char *kt = lds, *vt = lds + BN * TL::ROWB;
+    using FL = Fill<T, DT, BN>;
+    constexpr int TILE_B = BN * TL::ROWB;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];  // [stage][keys, values]
+    __shared__ __attribute__((aligned(16))) float bias[2][BN];       // 0, or -inf where the key does not count
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
     const int mtiles = (rw.R + SH::BM - 1) / SH::BM;
@@ -40,10 +46,56 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
     const int hk = id % rw.Hk, bz = id / rw.Hk;
 
     const RowAt at = row_at(rw, bz, hk, mt * SH::BM + wm * 32 + (lane & 31));
-    const int kb = bz;
-    const int len = clamped(a.keys.len, kb, a.keys.n);
+    const int len = clamped(a.keys.len, bz, a.keys.n);
     const int begin = split * a.chunk, end = min(len, begin + a.chunk);
     const int upto = a.tail ? len - (rw.M - 1 - at.i) : len;  // keys this row may see
+
+    const unsigned ksb = (unsigned)(a.keys.kr * sizeof(T)), vsb = (unsigned)(a.keys.vr * sizeof(T));  // row strides, bytes
+    const char *kp = (const char *)((const T *)a.keys.k + bz * a.keys.kb + hk * a.keys.kh);
+    const char *vp = (const char *)((const T *)a.keys.v + bz * a.keys.vb + hk * a.keys.vh);
+    const unsigned char *mask = a.keys.mask ? a.keys.mask + bz * a.keys.mask_b : nullptr;
+    const unsigned lds0 = lds_offset(lds);
+
+    unsigned ko[FL::N], vo[FL::N];  // the lane's places in a tile, as offsets from its first row
+#pragma unroll
+    for (int x = 0; x < FL::N; ++x) {
+        const unsigned c = FL::chunk(x, wave, lane, rw.D), r = FL::row(x, wave, lane);
+        ko[x] = c == DMA_OUT ? DMA_OUT : r * ksb + c;
+        vo[x] = c == DMA_OUT ? DMA_OUT : r * vsb + c;
+    }
+    // mask bytes of the tile after the next: for the rows the lane fetches, and (bit 8) for the key it writes the bias of
+    unsigned mb[FL::N + 1];
+    const auto look = [&](int n0) {
+        if (!mask)
+            return;
+#pragma unroll
+        for (int x = 0; x < FL::N; ++x) {
+            const int j = n0 + FL::row(x, wave, lane);
+            mb[x] = j < end ? mask[j] : 0;
+        }
+        const int j = n0 + tid;
+        mb[FL::N] = tid < BN && j < end ? mask[j] : 0;
+    };
+    const auto fetch = [&](int n0, int stage) {
+        const unsigned left = (unsigned)(end - n0);
+        const u32x4 kd = dma_buffer(kp + (long)n0 * ksb, (unsigned)min((unsigned long long)left * ksb, (unsigned long long)DMA_MOST));
+        const u32x4 vd = dma_buffer(vp + (long)n0 * vsb, (unsigned)min((unsigned long long)left * vsb, (unsigned long long)DMA_MOST));
+        const unsigned at0 = lds0 + stage * 2 * TILE_B;
+#pragma unroll
+        for (int x = 0; x < FL::N; ++x)
+            if (FL::on(x, wave)) {
+                const bool off = mask && !mb[x];
+                dma16(kd, off ? DMA_OUT : ko[x], at0 + FL::lds(x, wave));
+                dma16(vd, off ? DMA_OUT : vo[x], at0 + TILE_B + FL::lds(x, wave));
+            }
+        if (tid < BN && (mask || n0 + BN > end))
+            bias[stage][tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
+    };
+    if (begin < end) {
+        look(begin);
+        fetch(begin, 0);
+        look(begin + BN);
+    }
 
     x8<T> qf[2 * DT];
     load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
@@ -56,61 +108,47 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
             o[d][i] = 0.0f;
     float m = NEG_INF, l = 0.0f;
 
-    const T *kp = (const T *)a.keys.k + kb * a.keys.kb + hk * a.keys.kh;
-    const T *vp = (const T *)a.keys.v + kb * a.keys.vb + hk * a.keys.vh;
-    const unsigned char *mask = a.keys.mask ? a.keys.mask + kb * a.keys.mask_b : nullptr;
-    const auto counts = [mask](int j) { return !mask || mask[j]; };
-    const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
-
-    Stage<T, DT, BN, 256> sk, sv;
-    if (begin < end) {
-        sk.load(kp, a.keys.kr, begin, end, rw.D, tid, counts);
-        sv.load(vp, a.keys.vr, begin, end, rw.D, tid, counts);
-    }
-    for (int n0 = begin; n0 < end; n0 += BN) {
-        // which of this wave's keys count, as bits
-        const int w0 = n0 + wk * KT;
-        unsigned seen[NS];
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const int j = w0 + 32 * s + (lane & 31);
-            seen[s] = (unsigned)__ballot(j < end && counts(j));
-        }
-        __syncthreads();
-        sk.store(kt, tid);
-        sv.store(vt, tid);
-        __syncthreads();
+    int stage = 0;
+    for (int n0 = begin; n0 < end; n0 += BN, stage ^= 1) {
+        dma_wait();
+        __syncthreads();  // this tile is there, and nobody reads the other one any more
         if (n0 + BN < end) {
-            sk.load(kp, a.keys.kr, n0 + BN, end, rw.D, tid, counts);
-            sv.load(vp, a.keys.vr, n0 + BN, end, rw.D, tid, counts);
+            fetch(n0 + BN, stage ^ 1);
+            look(n0 + 2 * BN);
         }
-        bool any = false;
+        const char *kt = lds + stage * 2 * TILE_B, *vt = kt + TILE_B;
+        const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
+        const int w0 = n0 + wk * KT;
+
+        // a key that does not count starts at -inf (its features are zeros) and stays there
+        f32x16 sc[NS];
+        if (mask || n0 + BN > end) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage][wk * KT + 32 * s + 8 * x + 4 * half]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        sc[s][4 * x + j] = w[j];
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    sc[s][i] = 0.0f;
+        }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-            any |= seen[s] != 0;
-        if (!any)
-            continue;
-
-        f32x16 sc[NS];
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                sc[s][i] = 0.0f;
 #pragma unroll
             for (int t = 0; t < TL::KS; ++t)
                 sc[s] = mma(TL::row_frag(kt, rbase, wk * KT + 32 * s, t), qf[t], sc[s]);
-        }
-        // masked places: the score becomes -inf whatever it was
-        bool edge = a.tail && w0 + KT > len - rw.M + 1;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-            edge |= seen[s] != 0xffffffffu;
-        if (edge) {
+        if (a.tail && w0 + KT > len - rw.M + 1) {  // keys that only some of the rows see
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 const int left = upto - (w0 + 32 * s);
-                const unsigned bits = seen[s] & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+                const unsigned bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     sc[s][i] = bit_of(bits, half, i) ? sc[s][i] : NEG_INF;
@@ -158,7 +196,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && (WM == 4 || DT <= 2) ? 2 : 
 
     if constexpr (WK > 1) {  // join the waves' pieces of the key range, in wave order
         constexpr int PIECE = 64 * 16 * DT + 128;
-        static_assert((WK - 1) * WM * PIECE * 4 <= 2 * BN * TL::ROWB, "the join uses the tiles' memory");
+        static_assert((WK - 1) * WM * PIECE * 4 <= 4 * TILE_B, "the join uses the tiles' memory");
         float *pc = reinterpret_cast<float *>(lds);
         __syncthreads();
         if (wk > 0) {

@@ -198,35 +198,54 @@ __device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned total)
     return x * per + (x < rest ? x : rest) + at;
 }
 
-// registers on their way to an LDS tile: rows n0 .. n0 + BN - 1 of a strided matrix
-template <typename T, int DT, int BN, int NT>
-struct Stage {
-    using TL = Tile<T, DT>;
-    static constexpr int N = (BN * TL::NCH + NT - 1) / NT;
-    u32x4 r[N];
+// ---- memory -> LDS without registers -------------------------------------------------------------------------------------------
+// buffer_load_dwordx4 .. lds: lane i's 16 bytes land at M0 + 16 i, so one instruction fills 64 consecutive places of a tile and the
+// lanes choose which chunk goes where by their addresses (the swizzle of Tile).  Offsets are 32 bits relative to a 64-bit base
+// that moves with the tile; an offset outside the buffer delivers zeros, which is how rows past the end, rows that do not count
+// and padding features become zeros.  The compiler does not see these loads: dma_wait() comes before the barrier behind which a
+// tile is read.  M0 is reserved (never allocated; what the compiler uses it for, it sets right before), so it is no clobber.
+constexpr unsigned DMA_OUT = 0x80000000u;    // an offset that is outside every buffer
+constexpr unsigned DMA_MOST = 0x7fffffffu;   // bytes a buffer has at most
 
-    // p: row 0, feature 0; rows from `end` on, rows whose `on` says no, and padding features come as zeros
-    template <typename On>
-    __device__ __forceinline__ void load(const T *p, long stride, int n0, int end, int D, int tid, On on)
+__device__ __forceinline__ u32x4 dma_buffer(const void *base, unsigned bytes)
+{
+    const unsigned long long p = (unsigned long long)base;
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((unsigned)p);
+    r[1] = __builtin_amdgcn_readfirstlane((unsigned)(p >> 32)) & 0xffffu;
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = 0x00020000u;
+    return r;
+}
+__device__ __forceinline__ void dma16(u32x4 buffer, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ void dma4(u32x4 buffer, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_offset(const void *p) { return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)p; }
+
+// how the 4 waves of a workgroup fill a tile of BN rows: instruction x of a wave takes the places from 64 (4 x + wave) on
+template <typename T, int DT, int BN>
+struct Fill {
+    using TL = Tile<T, DT>;
+    static constexpr int WI = BN * TL::LC / 64;  // instructions of the tile
+    static constexpr int N = (WI + 3) / 4;       // of a wave
+    static constexpr int RPI = 64 / TL::LC;      // rows of an instruction
+    static_assert(BN * TL::LC % 64 == 0, "whole instructions");
+
+    static __device__ __forceinline__ bool on(int x, int wave) { return WI % 4 == 0 || 4 * x + wave < WI; }
+    static __device__ __forceinline__ int row(int x, int wave, int lane) { return (4 * x + wave) * RPI + lane / TL::LC; }
+    // the lane's chunk as a byte offset in its row; DMA_OUT where it is padding
+    static __device__ __forceinline__ unsigned chunk(int x, int wave, int lane, int D)
     {
-#pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int id = tid + x * NT, row = id / TL::NCH, c = id - row * TL::NCH;
-            u32x4 z = {0, 0, 0, 0};
-            if ((BN * TL::NCH % NT == 0 || row < BN) && n0 + row < end && c * TL::EPC < D && on(n0 + row))
-                z = *reinterpret_cast<const u32x4 *>(p + (long)(n0 + row) * stride + c * TL::EPC);
-            r[x] = z;
-        }
+        const int c = (lane % TL::LC) ^ TL::swz(row(x, wave, lane));
+        return c * TL::EPC < D ? 16u * c : DMA_OUT;
     }
-    __device__ __forceinline__ void store(char *tile, int tid) const
-    {
-#pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int id = tid + x * NT, row = id / TL::NCH, c = id - row * TL::NCH;
-            if (BN * TL::NCH % NT == 0 || row < BN)
-                *reinterpret_cast<u32x4 *>(tile + TL::place(row, c)) = r[x];
-        }
-    }
+    static __device__ __forceinline__ unsigned lds(int x, int wave) { return 1024u * (4 * x + wave); }
 };
 
 // weights of masked places: register i of a result tile is row 8 (i / 4) + 4 half + i % 4

@@ -359,7 +359,8 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * at the same time (other streams, graphs replayed side by side) need workspaces of their own.
  *
  * A gpx_view is a tensor [batch][row][head][dim]: base pointer and element strides of the first three axes, dim contiguous;
- * base and strides are multiples of 16 bytes, inputs may have zero strides, rows of an output must not overlap.  q, o, d_o, dq:
+ * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim) and are at most 2^22 elements
+ * apart, the heads of a group in q and d_o lie within 2^27; an input's batch and head strides may be zero.  q, o, d_o, dq:
  * [batch][nq][heads][dim]; k, v, dk, dv: [batch][nk][heads_kv][dim]; heads_kv divides heads, query head h reads key head
  * h / (heads / heads_kv).  dim: a multiple of 8 up to 128.  lse: [batch][heads][nq] floats, contiguous: log sum_j exp(score).
  *

@@ -26,6 +26,9 @@ def args(at, **kv):
     d.update(scalar=2, device=-1, batch=2, nq=3, nk=5, heads=4, heads_kv=2, dim=64, scale=0.125)
     for p in ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv", "k_own", "v_own"):
         d[p] = 4096
+    for p in NAMES:
+        if p in ("qr", "kr", "vr", "orow", "gr", "dqr", "dkr", "dvr", "kor", "vor"):
+            d[p] = 256
     d.update(kv)
     return at._ARGS.pack(*[d[n] for n in NAMES])
 
@@ -34,7 +37,8 @@ BAD = [(dict(scalar=3), -10), (dict(scalar=-1), -10), (dict(heads=3), -10), (dic
        (dict(dim=12), -10), (dict(dim=136), -10), (dict(batch=-1), -10), (dict(nq=-1), -10), (dict(nk=-1), -10), (dict(n_own=-1), -10),
        (dict(scale=0.0), -10), (dict(scale=-1.0), -10), (dict(scale=math.nan), -10), (dict(scale=math.inf), -10), (dict(scale=1e300), -10),
        (dict(nq=2 ** 31), -10), (dict(nk=2 ** 31), -10), (dict(batch=2 ** 20, nq=2 ** 20), -10), (dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1),
-       (dict(o=0), -1), (dict(lse=0), -1), (dict(q=4098), -10), (dict(kb=3), -10), (dict(vr=4), -10), (dict(qh=-8), -10), (dict(oh=1), -10)]
+       (dict(o=0), -1), (dict(lse=0), -1), (dict(q=4098), -10), (dict(kb=3), -10), (dict(vr=4), -10), (dict(qh=-8), -10), (dict(oh=1), -10),
+       (dict(kr=0), -10), (dict(vr=56), -10), (dict(kr=2 ** 22 + 8), -10), (dict(qh=2 ** 27), -10)]
 
 
 @pytest.mark.parametrize("kv,code", BAD, ids=lambda x: str(x))
