@@ -5,18 +5,6 @@
 #include "gpx_attend.hpp"
 #include "gpx_model.hpp"
 
-namespace gpx {
-// 32, 64 or 128 packed rows per workgroup; what is left of its 4 waves takes parts of the key range.  (fp32 rows of more than 64
-// features: 64 at least, four waves' tiles of keys would not leave a wave its registers.)
-int attend_block_rows(bool f32, int dim, int rows) { return rows <= 32 && !(f32 && dim > 64) ? 32 : rows <= 64 ? 64 : 128; }
-int attend_block_keys(bool f32, int dim, int rows)
-{
-    const int bm = attend_block_rows(f32, dim, rows);
-    return f32 ? 128 * 32 / bm : bm == 32 ? 128 : 64;
-}
-int attend_dkv_block_rows(bool f32) { return f32 ? 32 : 64; }
-}  // namespace gpx
-
 namespace {
 
 struct DeviceScope {  // the call runs on args->device; the caller's current device is restored
@@ -117,14 +105,16 @@ int check_data(const gpx_attend_args &a, int which)
     return GPX_OK;
 }
 
-// `pieces` of [0, n) in whole steps of `step`: enough workgroups to give every CU two where `blocks` alone would not give it one
-void cut(int64_t blocks, int64_t n, int step, int least, int cus, int *pieces, int *chunk)
+// `pieces` of [0, n) in whole steps of `step`, of at least `least` steps each: where `blocks` workgroups would leave CUs without
+// one, enough pieces that every CU has the `per_cu` it holds
+void cut(int64_t blocks, int64_t n, int step, int least, int cus, int per_cu, int *pieces, int *chunk)
 {
     int64_t p = 1;
+    const int64_t steps = std::max<int64_t>(1, (n + step - 1) / step);
     if (blocks < cus && blocks > 0)
-        p = std::min<int64_t>((2 * cus + blocks - 1) / blocks, n / ((int64_t)step * least));
+        p = std::min<int64_t>((int64_t)cus * per_cu / blocks, steps / least);
     p = std::max<int64_t>(p, 1);
-    const int64_t steps = std::max<int64_t>(1, (n + step - 1) / step), per = (steps + p - 1) / p;
+    const int64_t per = (steps + p - 1) / p;
     *chunk = (int)(per * step);
     *pieces = (int)((steps + per - 1) / per);
 }
@@ -134,46 +124,54 @@ int64_t blocks_of(int64_t rows, int64_t per) { return (rows + per - 1) / per; }
 struct Plan {
     int splits = 1, chunk = 0;          // forward / the shared context
     int own_splits = 0, own_chunk = 0;  // the own part
+    int mtiles = 1, own_mtiles = 1, ktiles = 1;  // workgroups along the rows, along the keys (backward)
     int k_splits = 1, k_chunk = 0;      // backward, dK dV: pieces of the rows
     size_t ml = 0, po = 0, pk = 0, pv = 0, total = 0;  // offsets into the workspace (ml: the row statistics in a backward call)
 };
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// Pieces of a forward or backward call cost one more launch that joins them (some 4 us, what 4 steps take): not below 6 steps
+// each.  A shared call joins its two parts anyway.
+constexpr int LEAST_STEPS = 6;
+
 Plan plan_of(const gpx_attend_args &a, int which, int cus)
 {
     Plan p;
     const int64_t G = a.heads / a.heads_kv;
-    const bool f32 = a.scalar == GPX_F32;
+    const int esz = elem_size(a), dt = attend_dt((int)a.dim);
     const size_t rid = (size_t)a.batch * a.nq * a.heads;
     if (which == GPX_ATTEND_SHARED) {
         const int R = (int)(a.batch * a.nq * G), Ro = (int)(a.nq * G);
+        const int wm = attend_wm(esz, dt, R), wo = attend_wm(esz, dt, 1);
+        p.mtiles = (int)blocks_of(R, 32 * wm), p.own_mtiles = (int)blocks_of(Ro, 32 * wo);
         if (a.nk > 0)
-            cut(blocks_of(R, attend_block_rows(f32, (int)a.dim, R)) * a.heads_kv, a.nk, attend_block_keys(f32, (int)a.dim, R), 2, cus, &p.splits, &p.chunk);
+            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), 1, cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
         else
             p.splits = 0;
         if (a.n_own > 0 || a.nk == 0)
-            cut(blocks_of(Ro, attend_block_rows(f32, (int)a.dim, Ro)) * a.heads_kv * a.batch, a.n_own, attend_block_keys(f32, (int)a.dim, Ro), 2, cus, &p.own_splits,
-                &p.own_chunk);
+            cut(p.own_mtiles * a.heads_kv * a.batch, a.n_own, attend_fwd_bn(esz, dt, wo), 1, cus, 1, &p.own_splits, &p.own_chunk);
         const size_t slots = p.splits + p.own_splits;
         p.ml = 0;
         p.po = up(slots * rid * sizeof(float2));
         p.total = p.po + slots * rid * a.dim * sizeof(float);
         return p;
     }
-    const int R = (int)(a.nq * G);
-    const int64_t blocks = blocks_of(R, attend_block_rows(f32, (int)a.dim, R)) * a.heads_kv * a.batch;
+    const int R = (int)(a.nq * G), wm = attend_wm(esz, dt, R);
+    p.mtiles = (int)blocks_of(R, 32 * wm);
+    const int64_t blocks = p.mtiles * a.heads_kv * a.batch;
     if (which == GPX_ATTEND_FORWARD) {
-        cut(blocks, a.nk, attend_block_keys(f32, (int)a.dim, R), 2, cus, &p.splits, &p.chunk);
+        cut(blocks, a.nk, attend_fwd_bn(esz, dt, wm), LEAST_STEPS, cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
         if (p.splits > 1) {
             p.po = up(p.splits * rid * sizeof(float2));
             p.total = p.po + p.splits * rid * a.dim * sizeof(float);
         }
         return p;
     }
-    cut(blocks, a.nk, 32 * (128 / attend_block_rows(f32, (int)a.dim, R)), 2, cus, &p.splits, &p.chunk);
-    cut(blocks_of(a.nk, ATTEND_DKV_KEYS) * a.heads_kv * a.batch, R, attend_dkv_block_rows(f32), 2, cus, &p.k_splits, &p.k_chunk);
-    size_t at = up(rid * sizeof(float2));
+    p.ktiles = (int)blocks_of(a.nk, ATTEND_DKV_KEYS);
+    cut(blocks, a.nk, attend_dq_bn(wm), LEAST_STEPS, cus, attend_dq_per_cu(esz, dt, wm), &p.splits, &p.chunk);
+    cut(p.ktiles * a.heads_kv * a.batch, R, attend_dkv_br(esz), LEAST_STEPS, cus, attend_dkv_per_cu(esz, dt), &p.k_splits, &p.k_chunk);
+    size_t at = up(2 * rid * sizeof(float));
     p.po = at;
     if (p.splits > 1)
         at = up(at + p.splits * rid * a.dim * sizeof(float));
@@ -209,7 +207,16 @@ AttendRows rows_of(const gpx_attend_args &a)
     r.D = (int)a.dim;
     r.R = r.M * r.G;
     r.grid_b = (int)a.batch;
+    r.by_m = DivBy((unsigned)std::max(1, r.M));
+    r.by_g = DivBy((unsigned)r.G);
+    r.by_hk = DivBy((unsigned)r.Hk);
     return r;
+}
+void set_grid(AttendFwd &f, int mtiles, int splits, int chunk)
+{
+    f.mtiles = mtiles, f.splits = splits, f.chunk = chunk;
+    f.by_mtiles = DivBy((unsigned)mtiles);
+    f.by_splits = DivBy((unsigned)std::max(1, splits));
 }
 AttendKeys keys_of(const gpx_view &k, const gpx_view &v, int64_t n, const int32_t *len, const uint8_t *mask, int64_t mask_b)
 {
@@ -283,7 +290,7 @@ extern "C" int gpx_attend(const gpx_attend_args *args)
     f.rows = rows_of(a);
     f.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
     f.c = (float)(a.scale * ATTEND_LOG2E);
-    f.splits = p.splits, f.chunk = p.chunk;
+    set_grid(f, p.mtiles, p.splits, p.chunk);
     f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
     f.lse = a.lse;
     f.slot_rows = (long)(a.batch * a.nq * a.heads);
@@ -317,28 +324,23 @@ extern "C" int gpx_attend_shared(const gpx_attend_args *args)
     f.slot_rows = (long)(a.batch * a.nq * a.heads);
     f.pml = (float2 *)((char *)a.workspace + p.ml);
     f.po = (float *)((char *)a.workspace + p.po);
-    // the shared context: the rows of the whole batch are rows of one grid entry
-    AttendFwd s = f;
-    s.rows = rows_of(a);
-    s.rows.R = (int)(a.batch * a.nq) * s.rows.G;
-    s.rows.grid_b = 1;
-    s.keys = keys_of(a.k, a.v, a.nk, nullptr, nullptr, 0);
-    s.splits = p.splits, s.chunk = p.chunk;
-    // the own part
-    AttendFwd w = f;
-    w.rows = rows_of(a);
-    w.keys = keys_of(a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
-    w.tail = 1;
-    w.splits = p.own_splits, w.chunk = p.own_chunk;
-    w.slot0 = p.splits;
+    // the shared context: the rows of the whole batch are rows of one grid entry; a context or own part of no rows has no
+    // workgroups
+    AttendPair w{f, f};
+    w.first.rows = w.second.rows = rows_of(a);
+    w.first.rows.R = (int)(a.batch * a.nq) * w.first.rows.G;
+    w.first.rows.grid_b = 1;
+    w.first.keys = keys_of(a.k, a.v, a.nk, nullptr, nullptr, 0);
+    set_grid(w.first, p.mtiles, p.splits, p.chunk);
+    w.second.keys = keys_of(a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
+    w.second.tail = 1;
+    w.second.slot0 = p.splits;
+    set_grid(w.second, p.own_mtiles, p.own_splits, p.own_chunk);
     return by_type(a, [&](auto t) {
         using T = decltype(t);
-        if (p.splits)
-            attend_launch_fwd<T>(s, (hipStream_t)a.stream);
-        if (p.own_splits)
-            attend_launch_fwd<T>(w, (hipStream_t)a.stream);
-        attend_launch_join<T>({f.po, f.pml, p.splits + p.own_splits, f.slot_rows, (int)a.nq, (int)a.heads, (int)a.dim, a.o.p, a.o.batch, a.o.row,
-                               a.o.head, a.lse},
+        attend_launch_pair<T>(w, (hipStream_t)a.stream);
+        attend_launch_join<T>({f.po, f.pml, p.splits + p.own_splits, f.slot_rows, (int)a.nq, (int)a.heads, (int)a.dim, a.o.p, a.o.batch,
+                               a.o.row, a.o.head, a.lse},
                               (hipStream_t)a.stream);
     });
 }
@@ -362,7 +364,11 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.dout = a.d_o.p, b.gb = a.d_o.batch, b.gr = a.d_o.row, b.gh = a.d_o.head;
     b.lse = a.lse;
     b.stat = (float *)((char *)a.workspace + p.ml);
-    b.div_g = DivBy((unsigned)b.rows.G);
+    b.mtiles = p.mtiles, b.ktiles = p.ktiles;
+    b.by_mtiles = DivBy((unsigned)std::max(1, p.mtiles));
+    b.by_ktiles = DivBy((unsigned)std::max(1, p.ktiles));
+    b.by_q_splits = DivBy((unsigned)p.splits);
+    b.by_k_splits = DivBy((unsigned)p.k_splits);
     b.dq = a.dq.p, b.dqb = a.dq.batch, b.dqr = a.dq.row, b.dqh = a.dq.head;
     b.dk = a.dk.p, b.dkb = a.dk.batch, b.dkr = a.dk.row, b.dkh = a.dk.head;
     b.dv = a.dv.p, b.dvb = a.dv.batch, b.dvr = a.dv.row, b.dvh = a.dv.head;

@@ -4,6 +4,7 @@
 
 namespace gpx {
 template void attend_launch_fwd<__bf16>(const AttendFwd &, hipStream_t);
+template void attend_launch_pair<__bf16>(const AttendPair &, hipStream_t);
 template void attend_launch_join<__bf16>(const AttendJoin &, hipStream_t);
 template void attend_launch_bwd<__bf16>(const AttendBwd &, hipStream_t);
 }  // namespace gpx

@@ -4,6 +4,7 @@
 
 namespace gpx {
 template void attend_launch_fwd<_Float16>(const AttendFwd &, hipStream_t);
+template void attend_launch_pair<_Float16>(const AttendPair &, hipStream_t);
 template void attend_launch_join<_Float16>(const AttendJoin &, hipStream_t);
 template void attend_launch_bwd<_Float16>(const AttendBwd &, hipStream_t);
 }  // namespace gpx

@@ -4,6 +4,7 @@
 
 namespace gpx {
 template void attend_launch_fwd<float>(const AttendFwd &, hipStream_t);
+template void attend_launch_pair<float>(const AttendPair &, hipStream_t);
 template void attend_launch_join<float>(const AttendJoin &, hipStream_t);
 template void attend_launch_bwd<float>(const AttendBwd &, hipStream_t);
 }  // namespace gpx

@@ -5,61 +5,20 @@
 // the packed rows do by themselves.  Two kernels, each forming p and dS again for its own sums (7 products instead of 5): dQ
 // with the rows held by the wave, dK and dV with the keys held by the wave.  No atomics: every sum has a fixed order.
 #pragma once
+#include <type_traits>
+
 #include "gpx_attend_tile.hpp"
 
 namespace gpx {
 namespace attend {
 
-// lse in log2 units (+inf where a row has no weights, so that every p is 0) and <dO, O>, one lane group of 16 per row
-template <typename T>
-__global__ __launch_bounds__(256) void attend_stat_kernel(AttendBwd a, long rows)
-{
-    const AttendRows &rw = a.rows;
-    const int sub = threadIdx.x & 15, H = rw.Hk * rw.G;
-    const long rid = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const bool on = rid < rows;
-    const int i = on ? (int)(rid % rw.M) : 0;
-    const long bh = on ? rid / rw.M : 0;
-    const int h = (int)(bh % H);
-    const long b = bh / H;
-    float s = 0.0f;
-    const bool valid = on && (!rw.len || i < rw.len[b]);
-    const int d = 8 * sub;
-    if (valid && d < rw.D) {
-        const x8<T> g = *reinterpret_cast<const x8<T> *>((const T *)a.dout + b * a.gb + i * a.gr + h * a.gh + d);
-        const x8<T> o = *reinterpret_cast<const x8<T> *>((const T *)a.o + b * a.ob + i * a.orow + h * a.oh + d);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            s += (float)g[j] * (float)o[j];
-    }
-#pragma unroll
-    for (int k = 8; k; k >>= 1)
-        s += __shfl_xor(s, k);
-    if (on && sub == 0) {
-        const float lse = valid ? a.lse[rid] : NEG_INF;
-        const bool none = lse == NEG_INF;
-        a.stat[rid] = none ? POS_INF : lse * 1.44269504088896f;
-        a.stat[rows + rid] = none ? 0.0f : s;
-    }
-}
-
 // dQ: waves and tiles as in the forward kernel.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
+// The first piece of the key range also leaves each row's statistics for the dK, dV kernel, which runs behind this one.
 template <typename T, int DT, int WM>
-struct DqShape {
-    static constexpr int WK = 4 / WM;
-    static constexpr int KT = 32;
-    static constexpr int BN = KT * WK;
-    static constexpr int BM = 32 * WM;
-    static constexpr int LDS = 4 * BN * Tile<T, DT>::ROWB;
-    static constexpr int PER_CU = LDS <= 80 * 1024 - 1024 && (sizeof(T) == 2 || DT <= 2) ? 2 : 1;
-};
-
-template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_kernel(AttendBwd a)
+__global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void attend_dq_kernel(AttendBwd a)
 {
     using TL = Tile<T, DT>;
-    using SH = DqShape<T, DT, WM>;
-    constexpr int BN = SH::BN, WK = SH::WK, KT = SH::KT;
+    constexpr int WK = 4 / WM, KT = 32, BN = attend_dq_bn(WM);
     using FL = Fill<T, DT, BN>;
     constexpr int TILE_B = BN * TL::ROWB;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];
@@ -68,15 +27,12 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
-    const int mtiles = (rw.R + SH::BM - 1) / SH::BM;
-    unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int mt = id % mtiles;
-    id /= mtiles;
-    const int split = id % a.q_splits;
-    id /= a.q_splits;
-    const int hk = id % rw.Hk, bz = id / rw.Hk;
+    const unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    const int u = a.by_mtiles(id), mt = id - u * a.mtiles;
+    const int us = rw.by_hk(u), hk = u - us * rw.Hk;
+    const int bz = a.by_q_splits(us), split = us - bz * a.q_splits;
 
-    const RowAt at = row_at(rw, bz, hk, mt * SH::BM + wm * 32 + (lane & 31));
+    const RowAt at = row_at(rw, bz, hk, mt * 32 * WM + wm * 32 + (lane & 31));
     const int len = clamped(a.keys.len, bz, a.keys.n);
     const int begin = split * a.q_chunk, end = min(len, begin + a.q_chunk);
 
@@ -110,14 +66,22 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
         const u32x4 kd = dma_buffer(kp + (long)n0 * ksb, (unsigned)min((unsigned long long)left * ksb, (unsigned long long)DMA_MOST));
         const u32x4 vd = dma_buffer(vp + (long)n0 * vsb, (unsigned)min((unsigned long long)left * vsb, (unsigned long long)DMA_MOST));
         const unsigned at0 = lds0 + stage * 2 * TILE_B;
+        if (mask) {
 #pragma unroll
-        for (int x = 0; x < FL::N; ++x)
-            if (FL::on(x, wave)) {
-                const bool off = mask && !mb[x];
-                dma16(kd, off ? DMA_OUT : ko[x], at0 + FL::lds(x, wave));
-                dma16(vd, off ? DMA_OUT : vo[x], at0 + TILE_B + FL::lds(x, wave));
-            }
-        if (tid < BN && (mask || n0 + BN > end))
+            for (int x = 0; x < FL::N; ++x)
+                if (FL::on(x, wave)) {
+                    dma16(kd, mb[x] ? ko[x] : DMA_OUT, at0 + FL::lds(x, wave));
+                    dma16(vd, mb[x] ? vo[x] : DMA_OUT, at0 + TILE_B + FL::lds(x, wave));
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < FL::N; ++x)
+                if (FL::on(x, wave)) {
+                    dma16(kd, ko[x], at0 + FL::lds(x, wave));
+                    dma16(vd, vo[x], at0 + TILE_B + FL::lds(x, wave));
+                }
+        }
+        if ((mask || n0 + BN > end) && tid < BN)
             bias[stage][tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
     };
     if (begin < end) {
@@ -129,11 +93,27 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
     x8<T> qf[2 * DT], gf[2 * DT];
     load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
     load_row_frags<T, DT>(gf, (const T *)a.dout + (at.valid ? at.b * a.gb + at.i * a.gr + at.h * a.gh : 0), at.valid, rw.D, lane);
+    // lse in log2 units (+inf where the row has no weights, so that every p is 0), and <dO, O>
     float lse = POS_INF, dd = 0.0f;
-    if (at.valid) {
+    {
+        x8<T> of[2 * DT];
+        load_row_frags<T, DT>(of, (const T *)a.o + (at.valid ? at.b * a.ob + at.i * a.orow + at.h * a.oh : 0), at.valid, rw.D, lane);
         const long rid = ((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i;
-        lse = a.stat[rid];
-        dd = a.stat[(long)rw.grid_b * rw.Hk * rw.G * rw.M + rid];
+        const float from = at.valid ? a.lse[rid] : NEG_INF;
+#pragma unroll
+        for (int t = 0; t < 2 * DT; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                dd += (float)gf[t][j] * (float)of[t][j];
+        dd = sum_both_halves(dd);
+        if (from != NEG_INF)
+            lse = from * 1.44269504088896f;
+        else
+            dd = 0.0f;
+        if (split == 0 && wk == 0 && half == 0 && at.exists) {
+            a.stat[rid] = lse;
+            a.stat[(long)rw.grid_b * rw.Hk * rw.G * rw.M + rid] = dd;
+        }
     }
 
     f32x16 dq[DT];
@@ -143,18 +123,15 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
         for (int i = 0; i < 16; ++i)
             dq[d][i] = 0.0f;
 
-    int stage = 0;
-    for (int n0 = begin; n0 < end; n0 += BN, stage ^= 1) {
-        dma_wait();
-        __syncthreads();
-        if (n0 + BN < end) {
-            fetch(n0 + BN, stage ^ 1);
-            look(n0 + 2 * BN);
-        }
-        const char *kt = lds + stage * 2 * TILE_B, *vt = kt + TILE_B;
-        const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
+    const auto step = [&](int stage, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const char *kt = lds, *vt = lds + TILE_B;
+        const int rbase = TL::row_base(lane) + stage * 2 * TILE_B, cbase = TL::col_base(lane) + stage * 2 * TILE_B;
         f32x16 sc, dp;
-        if (mask || n0 + BN > end) {  // -inf where the key does not count: its weight, and with it dS, is zero
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sc[i] = dp[i] = 0.0f;
+        if constexpr (EDGE) {  // -inf where the key does not count: its weight, and with it dS, is zero
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage][wk * KT + 8 * x + 4 * half]);
@@ -162,14 +139,7 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
                 for (int j = 0; j < 4; ++j)
                     sc[4 * x + j] = w[j];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                sc[i] = 0.0f;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            dp[i] = 0.0f;
 #pragma unroll
         for (int t = 0; t < TL::KS; ++t) {
             sc = mma(TL::row_frag(kt, rbase, wk * KT, t), qf[t], sc);
@@ -185,7 +155,22 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
             for (int d = 0; d < DT; ++d)
                 dq[d] = mma(TL::col_frag(kt, cbase, wk * KT + 16 * t, d), ds, dq[d]);
         }
-    }
+    };
+    const int plain = mask || end < begin ? begin : begin + (end - begin) / BN * BN;
+    int stage = 0;
+    const auto steps = [&](int from, int to, auto edge) {
+        for (int n0 = from; n0 < to; n0 += BN, stage ^= 1) {
+            dma_wait();
+            __syncthreads();
+            if (n0 + BN < end) {
+                fetch(n0 + BN, stage ^ 1);
+                look(n0 + 2 * BN);
+            }
+            step(stage, edge);
+        }
+    };
+    steps(begin, plain, std::false_type());
+    steps(plain, end, std::true_type());
     if constexpr (WK > 1) {
         constexpr int PIECE = 64 * 16 * DT;
         static_assert((WK - 1) * WM * PIECE * 4 <= 4 * TILE_B, "the join uses the tiles' memory");
@@ -245,16 +230,10 @@ __global__ __launch_bounds__(256, (DqShape<T, DT, WM>::PER_CU)) void attend_dq_k
 // dK, dV: 4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one
 // key, then dV^T += dO^T P and dK^T += Q^T dS.
 template <typename T, int DT>
-struct DkvShape {
-    static constexpr int BR = sizeof(T) == 2 ? 64 : 32;
-    static constexpr int PER_CU = sizeof(T) == 2 || DT <= 2 ? 2 : 1;
-};
-
-template <typename T, int DT>
-__global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_kernel(AttendBwd a)
+__global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void attend_dkv_kernel(AttendBwd a)
 {
     using TL = Tile<T, DT>;
-    constexpr int BR = DkvShape<T, DT>::BR;
+    constexpr int BR = attend_dkv_br(sizeof(T));
     using FL = Fill<T, DT, BR>;
     constexpr int TILE_B = BR * TL::ROWB;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];      // [stage][Q, dO]
@@ -268,13 +247,10 @@ __global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_ker
         return x;
     };
     const AttendRows &rw = a.rows;
-    const int ktiles = (a.keys.n + ATTEND_DKV_KEYS - 1) / ATTEND_DKV_KEYS;
-    unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int ktile = id % ktiles;
-    id /= ktiles;
-    const int split = id % a.k_splits;
-    id /= a.k_splits;
-    const int hk = id % rw.Hk, bz = id / rw.Hk;
+    const unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    const int u = a.by_ktiles(id), ktile = id - u * a.ktiles;
+    const int us = rw.by_hk(u), hk = u - us * rw.Hk;
+    const int bz = a.by_k_splits(us), split = us - bz * a.k_splits;
 
     const int len = clamped(a.keys.len, bz, a.keys.n);
     const auto counts_of = [&](int key) { return key < len && (!a.keys.mask || a.keys.mask[bz * a.keys.mask_b + key]); };
@@ -291,14 +267,14 @@ __global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_ker
     const unsigned qrb = (unsigned)(rw.qr * sizeof(T)), qhb = (unsigned)(rw.qh * sizeof(T));
     const unsigned grb = (unsigned)(a.gr * sizeof(T)), ghb = (unsigned)(a.gh * sizeof(T));
     const auto fetch = [&](int r0, int stage) {
-        const int n0 = a.div_g(r0), lane = lane_again();
+        const int n0 = rw.by_g(r0), lane = lane_again();
         const u32x4 qd = dma_buffer(qp + (long)n0 * rw.qr, DMA_MOST), gd = dma_buffer(gp + (long)n0 * a.gr, DMA_MOST);
         const unsigned at0 = lds0 + stage * 2 * TILE_B;
 #pragma unroll(DT > 2 ? 1 : FL::N)
         for (int x = 0; x < FL::N; ++x)
             if (FL::on(x, wave)) {
                 const int r = r0 + FL::row(x, wave, lane);
-                const int n = a.div_g(r), g = r - n * rw.G;
+                const int n = rw.by_g(r), g = r - n * rw.G;
                 const unsigned c = FL::chunk(x, wave, lane, rw.D);
                 const bool off = r >= end || c == DMA_OUT;
                 dma16(qd, off ? DMA_OUT : (unsigned)(n - n0) * qrb + g * qhb + c, at0 + FL::lds(x, wave));
@@ -306,7 +282,7 @@ __global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_ker
             }
         if (wave < 2) {  // a row past the end gets zeros, and has zeros for Q and dO: it adds nothing
             const int r = r0 + lane;
-            const int n = a.div_g(r), g = r - n * rw.G;
+            const int n = rw.by_g(r), g = r - n * rw.G;
             const u32x4 sd = dma_buffer(sp + wave * stats + n0, DMA_MOST);
             dma4(sd, lane < BR && r < end ? 4u * (g * rw.M + (n - n0)) : DMA_OUT, stat0 + (stage * 2 + wave) * 256);
         }
@@ -422,28 +398,40 @@ __global__ __launch_bounds__(256, (DkvShape<T, DT>::PER_CU)) void attend_dkv_ker
         }
 }
 
-// out[row] = f sum_s p[s][row], in slot order; rows of D values, four per lane.  Row -> (batch, n, head) by the strides.
+// out[row] = f sum_s p[s][row], in slot order; rows of D values, four per lane.  Row -> (batch, n, head) by the strides.  Up to
+// three of them (dQ, dK, dV) in one launch.
 struct AttendSum {
-    const float *p;
-    int slots, D, n, H;  // row = (b n + i) H + h  or, head_first, (b H + h) n + i
-    long rows;
-    int head_first;
-    float f;
-    void *out;
-    long ob, orow, oh;
+    const float *p = nullptr;
+    int slots = 0, n = 1, H = 1;  // row = (b n + i) H + h or, head_first, (b H + h) n + i
+    long rows = 0;
+    int head_first = 0;
+    float f = 1;
+    void *out = nullptr;
+    long ob = 0, orow = 0, oh = 0;
+    unsigned blocks = 0;
+};
+struct AttendSums {
+    AttendSum s[3];
+    int D;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void attend_sum_kernel(AttendSum a)
+__global__ __launch_bounds__(256) void attend_sum_kernel(AttendSums all)
 {
-    const int q = a.D >> 2;
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    unsigned at = blockIdx.x;
+    int w = 0;
+    while (w < 2 && at >= all.s[w].blocks)
+        at -= all.s[w++].blocks;
+    const AttendSum &a = all.s[w];
+    const int q = all.D >> 2;
+    const long id = (long)at * 256 + threadIdx.x;
     if (id >= a.rows * q)
         return;
     const long row = id / q;
     const int d = 4 * (int)(id - row * q);
     f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
     for (int k = 0; k < a.slots; ++k)
-        s += *reinterpret_cast<const f32x4 *>(a.p + ((long)k * a.rows + row) * a.D + d);
+        s += *reinterpret_cast<const f32x4 *>(a.p + ((long)k * a.rows + row) * all.D + d);
     long b, i, h;
     if (a.head_first) {
         i = row % a.n;
@@ -454,44 +442,30 @@ __global__ __launch_bounds__(256) void attend_sum_kernel(AttendSum a)
         i = row / a.H % a.n;
         b = row / a.H / a.n;
     }
-    x4<T> w;
+    x4<T> v;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        w[j] = (T)(s[j] * a.f);
-    *reinterpret_cast<x4<T> *>((T *)a.out + b * a.ob + i * a.orow + h * a.oh + d) = w;
+        v[j] = (T)(s[j] * a.f);
+    *reinterpret_cast<x4<T> *>((T *)a.out + b * a.ob + i * a.orow + h * a.oh + d) = v;
 }
 
-template <typename T, int DT, int WM>
-void launch_dq_shape(const AttendBwd &a, hipStream_t st)
-{
-    const int mtiles = (a.rows.R + 32 * WM - 1) / (32 * WM);
-    const unsigned grid = (unsigned)((long)mtiles * a.q_splits * a.rows.Hk * a.rows.grid_b);
-    hipLaunchKernelGGL((attend_dq_kernel<T, DT, WM>), dim3(grid), dim3(256), 0, st, a);
-}
 template <typename T, int DT>
 void launch_bwd_dim(const AttendBwd &a, hipStream_t st)
 {
-    if (a.rows.R > 0 && a.rows.M > 0) {
-        switch (attend_block_rows(sizeof(T) == 4, a.rows.D, a.rows.R)) {
-        case 32:
-        if constexpr (sizeof(T) == 2 || DT <= 2)
-            launch_dq_shape<T, DT, 1>(a, st);
-        break;
-        case 64: launch_dq_shape<T, DT, 2>(a, st); break;
-        default: launch_dq_shape<T, DT, 4>(a, st); break;
+    const dim3 block(256);
+    if (a.rows.R > 0) {
+        const dim3 grid((unsigned)(a.mtiles * a.q_splits * a.rows.Hk * a.rows.grid_b));
+        switch (attend_wm(sizeof(T), DT, a.rows.R)) {
+        case 1:
+            if constexpr (attend_wm(sizeof(T), DT, 1) == 1)
+                hipLaunchKernelGGL((attend_dq_kernel<T, DT, 1>), grid, block, 0, st, a);
+            break;
+        case 2: hipLaunchKernelGGL((attend_dq_kernel<T, DT, 2>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((attend_dq_kernel<T, DT, 4>), grid, block, 0, st, a); break;
         }
     }
-    const int ktiles = (a.keys.n + ATTEND_DKV_KEYS - 1) / ATTEND_DKV_KEYS;
-    const unsigned grid = (unsigned)((long)ktiles * a.k_splits * a.rows.Hk * a.rows.grid_b);
-    if (grid)
-        hipLaunchKernelGGL((attend_dkv_kernel<T, DT>), dim3(grid), dim3(256), 0, st, a);
-}
-template <typename T>
-void launch_sum(const AttendSum &s, hipStream_t st)
-{
-    const long lanes = s.rows * (s.D / 4);
-    if (lanes)
-        hipLaunchKernelGGL((attend_sum_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, s);
+    if (a.keys.n > 0)
+        hipLaunchKernelGGL((attend_dkv_kernel<T, DT>), dim3((unsigned)(a.ktiles * a.k_splits * a.rows.Hk * a.rows.grid_b)), block, 0, st, a);
 }
 
 }  // namespace attend
@@ -500,23 +474,31 @@ template <typename T>
 void attend_launch_bwd(const AttendBwd &a, hipStream_t st)
 {
     const AttendRows &rw = a.rows;
-    const int H = rw.Hk * rw.G;
-    const long rows = (long)rw.grid_b * rw.M * H;
-    if (rows)
-        hipLaunchKernelGGL((attend::attend_stat_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a, rows);
-    switch ((rw.D + 31) / 32) {
+    switch (attend_dt(rw.D)) {
     case 1: attend::launch_bwd_dim<T, 1>(a, st); break;
     case 2: attend::launch_bwd_dim<T, 2>(a, st); break;
     case 3: attend::launch_bwd_dim<T, 3>(a, st); break;
     default: attend::launch_bwd_dim<T, 4>(a, st); break;
     }
-    if (a.pq)
-        attend::launch_sum<T>({a.pq, a.q_splits, rw.D, rw.M, H, rows, 0, a.scale, a.dq, a.dqb, a.dqr, a.dqh}, st);
-    if (a.pk) {
-        const long kr = (long)rw.grid_b * rw.Hk * a.keys.n;
-        attend::launch_sum<T>({a.pk, a.k_splits, rw.D, a.keys.n, rw.Hk, kr, 1, a.scale, a.dk, a.dkb, a.dkr, a.dkh}, st);
-        attend::launch_sum<T>({a.pv, a.k_splits, rw.D, a.keys.n, rw.Hk, kr, 1, 1.0f, a.dv, a.dvb, a.dvr, a.dvh}, st);
+    attend::AttendSums s;
+    s.D = rw.D;
+    if (a.pq) {
+        attend::AttendSum &q = s.s[0];
+        q.p = a.pq, q.slots = a.q_splits, q.n = rw.M, q.H = rw.Hk * rw.G, q.rows = (long)rw.grid_b * rw.M * q.H, q.f = a.scale;
+        q.out = a.dq, q.ob = a.dqb, q.orow = a.dqr, q.oh = a.dqh;
     }
+    if (a.pk) {
+        attend::AttendSum &k = s.s[1], &v = s.s[2];
+        k.slots = a.k_splits, k.n = a.keys.n, k.H = rw.Hk, k.rows = (long)rw.grid_b * rw.Hk * a.keys.n, k.head_first = 1;
+        v = k;
+        k.p = a.pk, k.f = a.scale, k.out = a.dk, k.ob = a.dkb, k.orow = a.dkr, k.oh = a.dkh;
+        v.p = a.pv, v.out = a.dv, v.ob = a.dvb, v.orow = a.dvr, v.oh = a.dvh;
+    }
+    unsigned grid = 0;
+    for (attend::AttendSum &x : s.s)
+        grid += x.blocks = (unsigned)((x.rows * (rw.D / 4) + 255) / 256);
+    if (grid)
+        hipLaunchKernelGGL((attend::attend_sum_kernel<T>), dim3(grid), dim3(256), 0, st, s);
 }
 
 }  // namespace gpx

@@ -1,6 +1,8 @@
 // gpx_attend_kernel.hpp -- the kernels of gpx_attend / gpx_attend_shared (forward) and gpx_attend_backward, as templates over
 // the element type; gpx_attend_f32.hip, _f16.hip and _bf16.hip instantiate them.
 #pragma once
+#include <type_traits>
+
 #include "gpx_attend_tile.hpp"
 
 namespace gpx {
@@ -12,40 +14,23 @@ namespace attend {
 // register per lane, and S^T turns into the operand of O^T = V^T P^T without leaving the lane (gpx_attend_tile.hpp).
 // Keys and values are read from memory once per 32 WM rows, as tiles of BN rows, two of them in LDS: while one is worked on the
 // next is on its way.
-template <typename T, int DT, int WM>
-struct FwdShape {
-    static constexpr int WK = 4 / WM;
-    static constexpr int KT = sizeof(T) == 2 && WK == 1 ? 64 : 32;  // keys of a wave per step
-    static constexpr int BN = KT * WK;
-    static constexpr int BM = 32 * WM;
-    static constexpr int LDS = 4 * BN * Tile<T, DT>::ROWB;
-    // workgroups a CU has room for (its 160 KB of LDS, and two waves per SIMD where the registers allow it)
-    static constexpr int PER_CU = LDS <= 80 * 1024 - 1024 ? 2 : 1;
-};
-
-template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd_kernel(AttendFwd a)
+// STAGES == 1 has one tile at a time (the own part of a shared call: short ranges, many workgroups a CU).
+template <typename T, int DT, int WM, int STAGES>
+__device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, float *bias, unsigned id)
 {
     using TL = Tile<T, DT>;
-    using SH = FwdShape<T, DT, WM>;
-    constexpr int BN = SH::BN, WK = SH::WK, KT = SH::KT, NS = KT / 32;
+    constexpr int WK = 4 / WM, KT = attend_fwd_kt(sizeof(T), DT, WM), NS = KT / 32, BN = KT * WK;
     using FL = Fill<T, DT, BN>;
-    constexpr int TILE_B = BN * TL::ROWB;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];  // [stage][keys, values]
-    __shared__ __attribute__((aligned(16))) float bias[2][BN];       // 0, or -inf where the key does not count
+    constexpr int TILE_B = BN * TL::ROWB;  // lds: [stage][keys, values]; bias: [stage][BN], 0 or -inf where the key does not count
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
-    const int mtiles = (rw.R + SH::BM - 1) / SH::BM;
-    unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int mt = id % mtiles;
-    id /= mtiles;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int hk = id % rw.Hk, bz = id / rw.Hk;
+    const int u = a.by_mtiles(id), mt = id - u * a.mtiles;
+    const int us = rw.by_hk(u), hk = u - us * rw.Hk;
+    const int bz = a.by_splits(us), split = us - bz * a.splits;
 
-    const RowAt at = row_at(rw, bz, hk, mt * SH::BM + wm * 32 + (lane & 31));
+    const RowAt at = row_at(rw, bz, hk, mt * 32 * WM + wm * 32 + (lane & 31));
     const int len = clamped(a.keys.len, bz, a.keys.n);
     const int begin = split * a.chunk, end = min(len, begin + a.chunk);
     const int upto = a.tail ? len - (rw.M - 1 - at.i) : len;  // keys this row may see
@@ -63,7 +48,7 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
         ko[x] = c == DMA_OUT ? DMA_OUT : r * ksb + c;
         vo[x] = c == DMA_OUT ? DMA_OUT : r * vsb + c;
     }
-    // mask bytes of the tile after the next: for the rows the lane fetches, and (bit 8) for the key it writes the bias of
+    // mask bytes of the next tile to fetch: for the rows the lane fetches, and for the key it writes the bias of
     unsigned mb[FL::N + 1];
     const auto look = [&](int n0) {
         if (!mask)
@@ -81,15 +66,23 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
         const u32x4 kd = dma_buffer(kp + (long)n0 * ksb, (unsigned)min((unsigned long long)left * ksb, (unsigned long long)DMA_MOST));
         const u32x4 vd = dma_buffer(vp + (long)n0 * vsb, (unsigned)min((unsigned long long)left * vsb, (unsigned long long)DMA_MOST));
         const unsigned at0 = lds0 + stage * 2 * TILE_B;
+        if (mask) {
 #pragma unroll
-        for (int x = 0; x < FL::N; ++x)
-            if (FL::on(x, wave)) {
-                const bool off = mask && !mb[x];
-                dma16(kd, off ? DMA_OUT : ko[x], at0 + FL::lds(x, wave));
-                dma16(vd, off ? DMA_OUT : vo[x], at0 + TILE_B + FL::lds(x, wave));
-            }
-        if (tid < BN && (mask || n0 + BN > end))
-            bias[stage][tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
+            for (int x = 0; x < FL::N; ++x)
+                if (FL::on(x, wave)) {
+                    dma16(kd, mb[x] ? ko[x] : DMA_OUT, at0 + FL::lds(x, wave));
+                    dma16(vd, mb[x] ? vo[x] : DMA_OUT, at0 + TILE_B + FL::lds(x, wave));
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < FL::N; ++x)
+                if (FL::on(x, wave)) {
+                    dma16(kd, ko[x], at0 + FL::lds(x, wave));
+                    dma16(vd, vo[x], at0 + TILE_B + FL::lds(x, wave));
+                }
+        }
+        if ((mask || a.tail || n0 + BN > end) && tid < BN)
+            bias[stage * BN + tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
     };
     if (begin < end) {
         look(begin);
@@ -108,50 +101,43 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
             o[d][i] = 0.0f;
     float m = NEG_INF, l = 0.0f;
 
-    int stage = 0;
-    for (int n0 = begin; n0 < end; n0 += BN, stage ^= 1) {
-        dma_wait();
-        __syncthreads();  // this tile is there, and nobody reads the other one any more
-        if (n0 + BN < end) {
-            fetch(n0 + BN, stage ^ 1);
-            look(n0 + 2 * BN);
-        }
-        const char *kt = lds + stage * 2 * TILE_B, *vt = kt + TILE_B;
-        const int rbase = TL::row_base(lane), cbase = TL::col_base(lane);
-        const int w0 = n0 + wk * KT;
-
-        // a key that does not count starts at -inf (its features are zeros) and stays there
+    // one tile; EDGE: some of its keys do not count, or not for every row
+    const auto step = [&](int n0, int stage, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const char *kt = lds, *vt = lds + TILE_B;
+        const int rbase = TL::row_base(lane) + stage * 2 * TILE_B, cbase = TL::col_base(lane) + stage * 2 * TILE_B;
         f32x16 sc[NS];
-        if (mask || n0 + BN > end) {
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                sc[s][i] = 0.0f;
+            if constexpr (EDGE) {  // a key that does not count starts at -inf (its features are zeros) and stays there
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage][wk * KT + 32 * s + 8 * x + 4 * half]);
+                    const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage * BN + wk * KT + 32 * s + 8 * x + 4 * half]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         sc[s][4 * x + j] = w[j];
                 }
-        } else {
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    sc[s][i] = 0.0f;
+            }
         }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int t = 0; t < TL::KS; ++t)
                 sc[s] = mma(TL::row_frag(kt, rbase, wk * KT + 32 * s, t), qf[t], sc[s]);
-        if (a.tail && w0 + KT > len - rw.M + 1) {  // keys that only some of the rows see
+        if constexpr (EDGE) {
+            const int w0 = n0 + wk * KT;
+            if (a.tail && w0 + KT > len - rw.M + 1) {  // keys that only some of the rows see
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int left = upto - (w0 + 32 * s);
-                const unsigned bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                for (int s = 0; s < NS; ++s) {
+                    const int left = upto - (w0 + 32 * s);
+                    const unsigned bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    sc[s][i] = bit_of(bits, half, i) ? sc[s][i] : NEG_INF;
+                    for (int i = 0; i < 16; ++i)
+                        sc[s][i] = bit_of(bits, half, i) ? sc[s][i] : NEG_INF;
+                }
             }
         }
         float top = NEG_INF;
@@ -160,10 +146,11 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 top = fmaxf(top, sc[s][i]);
-        top = fmaxf(top, other_half(top)) * a.c;
+        top = max_both_halves(top) * a.c;
         // The running maximum need not be the true one: sums in 32 bits and weights of up to 2^8 lose nothing, so it is
-        // raised (and what is summed so far rescaled) only when the new one is more than 8 above it.
-        if (__any(top > m + 8.0f || (m == NEG_INF && top > NEG_INF))) {
+        // raised (and what is summed so far rescaled) only when the new one is more than 8 above it.  (A row without a key
+        // so far has m = -inf, and is raised by any.)
+        if (__any(top > m + 8.0f)) {
             const float mn = fmaxf(m, top);
             const float f = mn == NEG_INF ? 1.0f : exp2_(m - mn);
             m = mn;
@@ -174,7 +161,7 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
                 for (int i = 0; i < 16; ++i)
                     o[d][i] *= f;
         }
-        const float sub = m == NEG_INF ? 0.0f : m;
+        const float sub = EDGE && m == NEG_INF ? 0.0f : m;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -191,12 +178,35 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
                 for (int d = 0; d < DT; ++d)
                     o[d] = mma(TL::col_frag(vt, cbase, wk * KT + 32 * s + 16 * t, d), p, o[d]);
             }
-    }
-    l += other_half(l);
+    };
+
+    const int plain = mask || a.tail || end < begin ? begin : begin + (end - begin) / BN * BN;  // tiles before are whole
+    int stage = 0;
+    const auto steps = [&](int from, int to, auto edge) {
+        for (int n0 = from; n0 < to; n0 += BN) {
+            dma_wait();
+            __syncthreads();  // this tile is there, and nobody reads the other one any more
+            if (STAGES == 2 && n0 + BN < end) {
+                fetch(n0 + BN, stage ^ 1);
+                look(n0 + 2 * BN);
+            }
+            step(n0, stage, edge);
+            if (STAGES == 2) {
+                stage ^= 1;
+            } else if (n0 + BN < end) {
+                __syncthreads();
+                fetch(n0 + BN, 0);
+                look(n0 + 2 * BN);
+            }
+        }
+    };
+    steps(begin, plain, std::false_type());
+    steps(plain, end, std::true_type());
+    l = sum_both_halves(l);
 
     if constexpr (WK > 1) {  // join the waves' pieces of the key range, in wave order
         constexpr int PIECE = 64 * 16 * DT + 128;
-        static_assert((WK - 1) * WM * PIECE * 4 <= 4 * TILE_B, "the join uses the tiles' memory");
+        static_assert((WK - 1) * WM * PIECE * 4 <= STAGES * 2 * TILE_B, "the join uses the tiles' memory");
         float *pc = reinterpret_cast<float *>(lds);
         __syncthreads();
         if (wk > 0) {
@@ -268,42 +278,84 @@ __global__ __launch_bounds__(256, (FwdShape<T, DT, WM>::PER_CU)) void attend_fwd
         }
 }
 
-// One wave per row: the pieces' maxima and sums (a lane each, 64 at a time), then the pieces' sums weighted by them.
+template <typename T, int DT, int WM>
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_fwd_kernel(AttendFwd a)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[attend_fwd_lds(sizeof(T), DT, WM, 2)];
+    __shared__ __attribute__((aligned(16))) float bias[2 * attend_fwd_bn(sizeof(T), DT, WM)];
+    attend_fwd_block<T, DT, WM, 2>(a, lds, bias, xcd_order(blockIdx.x, gridDim.x));
+}
+
+// Both parts of a shared call in one launch.  The own part has few rows per workgroup whatever the first has.
+template <typename T, int DT>
+constexpr int own_wm() { return attend_wm(sizeof(T), DT, 1); }
+template <typename T, int DT, int WM>
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_pair_kernel(AttendPair a)
+{
+    constexpr int OWN = own_wm<T, DT>();
+    constexpr int A = attend_fwd_lds(sizeof(T), DT, WM, 2), B = attend_fwd_lds(sizeof(T), DT, OWN, 1);
+    constexpr int NA = 2 * attend_fwd_bn(sizeof(T), DT, WM), NB = attend_fwd_bn(sizeof(T), DT, OWN);
+    __shared__ __attribute__((aligned(1024))) char lds[A > B ? A : B];
+    __shared__ __attribute__((aligned(16))) float bias[NA > NB ? NA : NB];
+    const unsigned n = a.first.mtiles * a.first.splits * a.first.rows.Hk;  // (one grid entry)
+    if (blockIdx.x < n)
+        attend_fwd_block<T, DT, WM, 2>(a.first, lds, bias, xcd_order(blockIdx.x, n));
+    else
+        attend_fwd_block<T, DT, OWN, 1>(a.second, lds, bias, xcd_order(blockIdx.x - n, gridDim.x - n));
+}
+
+// One wave per row: the pieces' maxima and sums (a lane each, 64 at a time), then the pieces' sums weighted by them, the two halves
+// of the wave taking every other piece, four values a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendJoin a)
 {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     const long rid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (rid >= a.slot_rows)
         return;
-    float top = NEG_INF;
-    for (int s = lane; s < a.slots; s += 64)
-        top = fmaxf(top, a.pml[s * a.slot_rows + rid].x);
-#pragma unroll
-    for (int k = 32; k; k >>= 1)
-        top = fmaxf(top, __shfl_xor(top, k));
-    const int d = 2 * lane;  // D is at most 128
-    float l = 0.0f, x = 0.0f, y = 0.0f;
+    const int d = 4 * (lane & 31);  // D is at most 128
+    const float *po = a.po + rid * a.D + (d < a.D ? d : 0);
+    const long step = a.slot_rows * a.D;
+    float top = NEG_INF, l = 0.0f;
+    f32x4 x = {0, 0, 0, 0};
     for (int s0 = 0; s0 < a.slots; s0 += 64) {
-        float w = 0.0f;
-        if (s0 + lane < a.slots) {
-            const float2 ml = a.pml[(long)(s0 + lane) * a.slot_rows + rid];
-            w = ml.y == 0.0f ? 0.0f : exp2_(ml.x - top);
-            l += ml.y == 0.0f ? 0.0f : w * ml.y;
-        }
+        float2 ml = make_float2(NEG_INF, 0.0f);
+        if (s0 + lane < a.slots)
+            ml = a.pml[(s0 + lane) * a.slot_rows + rid];
+        float mn = ml.x;
+#pragma unroll
+        for (int k = 32; k; k >>= 1)
+            mn = fmaxf(mn, __shfl_xor(mn, k));
+        mn = fmaxf(mn, top);
+        const float f = top == NEG_INF ? 0.0f : exp2_(top - mn);
+        top = mn;
+        const float w = ml.y == 0.0f ? 0.0f : exp2_(ml.x - mn);
+        l = l * f + w * ml.y;
+        x *= f;
         const int k = min(64, a.slots - s0);
-        for (int s = 0; s < k; ++s) {
-            const float ws = __shfl(w, s);
-            if (ws != 0.0f && d < a.D) {
-                const float2 p = *reinterpret_cast<const float2 *>(a.po + ((s0 + s) * a.slot_rows + rid) * a.D + d);
-                x += ws * p.x;
-                y += ws * p.y;
+        for (int s = 0; s < k; s += 8) {
+            f32x4 p[4];
+            float ws[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int mine = s + 2 * y + half, in = min(mine, k - 1);
+                p[y] = *reinterpret_cast<const f32x4 *>(po + (s0 + in) * step);
+                ws[y] = __shfl(w, in);
+                ws[y] = mine < k ? ws[y] : 0.0f;
             }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[j] += ws[y] == 0.0f ? 0.0f : ws[y] * p[y][j];  // what a piece without weights has there was never written
         }
     }
 #pragma unroll
     for (int k = 32; k; k >>= 1)
         l += __shfl_xor(l, k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        x[j] = sum_both_halves(x[j]);
     const int h = (int)(rid % a.H);
     const long n = rid / a.H;
     const int i = (int)(n % a.M);
@@ -311,31 +363,40 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendJoin a)
     const bool none = l == 0.0f;
     if (lane == 0)
         a.lse[(b * a.H + h) * a.M + i] = none ? NEG_INF : (top + log2_(l)) * 0.693147180559945f;
-    if (d < a.D) {
-        T *o = (T *)a.o + b * a.ob + i * a.orow + h * a.oh + d;
+    if (half == 0 && d < a.D) {
         const float inv = none ? 0.0f : 1.0f / l;
-        o[0] = none ? (T)0.0f : (T)(x * inv);
-        o[1] = none ? (T)0.0f : (T)(y * inv);
+        x4<T> w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = none ? (T)0.0f : (T)(x[j] * inv);
+        *reinterpret_cast<x4<T> *>((T *)a.o + b * a.ob + i * a.orow + h * a.oh + d) = w;
     }
 }
 
-template <typename T, int DT, int WM>
-void launch_fwd_shape(const AttendFwd &a, hipStream_t st)
-{
-    const int mtiles = (a.rows.R + 32 * WM - 1) / (32 * WM);
-    const unsigned grid = (unsigned)((long)mtiles * a.splits * a.rows.Hk * a.rows.grid_b);
-    hipLaunchKernelGGL((attend_fwd_kernel<T, DT, WM>), dim3(grid), dim3(256), 0, st, a);
-}
 template <typename T, int DT>
 void launch_fwd_dim(const AttendFwd &a, hipStream_t st)
 {
-    switch (attend_block_rows(sizeof(T) == 4, a.rows.D, a.rows.R)) {
-    case 32:
-        if constexpr (sizeof(T) == 2 || DT <= 2)
-            launch_fwd_shape<T, DT, 1>(a, st);
+    const dim3 grid((unsigned)a.blocks()), block(256);
+    switch (attend_wm(sizeof(T), DT, a.rows.R)) {
+    case 1:
+        if constexpr (own_wm<T, DT>() == 1)
+            hipLaunchKernelGGL((attend_fwd_kernel<T, DT, 1>), grid, block, 0, st, a);
         break;
-    case 64: launch_fwd_shape<T, DT, 2>(a, st); break;
-    default: launch_fwd_shape<T, DT, 4>(a, st); break;
+    case 2: hipLaunchKernelGGL((attend_fwd_kernel<T, DT, 2>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((attend_fwd_kernel<T, DT, 4>), grid, block, 0, st, a); break;
+    }
+}
+template <typename T, int DT>
+void launch_pair_dim(const AttendPair &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)(a.first.blocks() + a.second.blocks())), block(256);
+    switch (attend_wm(sizeof(T), DT, a.first.rows.R)) {
+    case 1:
+        if constexpr (own_wm<T, DT>() == 1)
+            hipLaunchKernelGGL((attend_pair_kernel<T, DT, 1>), grid, block, 0, st, a);
+        break;
+    case 2: hipLaunchKernelGGL((attend_pair_kernel<T, DT, 2>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((attend_pair_kernel<T, DT, 4>), grid, block, 0, st, a); break;
     }
 }
 
@@ -344,11 +405,21 @@ void launch_fwd_dim(const AttendFwd &a, hipStream_t st)
 template <typename T>
 void attend_launch_fwd(const AttendFwd &a, hipStream_t st)
 {
-    switch ((a.rows.D + 31) / 32) {
+    switch (attend_dt(a.rows.D)) {
     case 1: return attend::launch_fwd_dim<T, 1>(a, st);
     case 2: return attend::launch_fwd_dim<T, 2>(a, st);
     case 3: return attend::launch_fwd_dim<T, 3>(a, st);
     default: return attend::launch_fwd_dim<T, 4>(a, st);
+    }
+}
+template <typename T>
+void attend_launch_pair(const AttendPair &a, hipStream_t st)
+{
+    switch (attend_dt(a.first.rows.D)) {
+    case 1: return attend::launch_pair_dim<T, 1>(a, st);
+    case 2: return attend::launch_pair_dim<T, 2>(a, st);
+    case 3: return attend::launch_pair_dim<T, 3>(a, st);
+    default: return attend::launch_pair_dim<T, 4>(a, st);
     }
 }
 template <typename T>

@@ -50,7 +50,25 @@ __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x
 constexpr float NEG_INF = -__builtin_huge_valf(), POS_INF = __builtin_huge_valf();
 
 // lanes l and l ^ 32 hold the two halves of every column
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+__device__ __forceinline__ void both_halves(float x, float &a, float &b)  // a: the lower lanes' value, b: the upper lanes'
+{
+    unsigned u = __builtin_bit_cast(unsigned, x), w = u;
+    // (the builtin hands back its first result twice; two wait states after the instruction that wrote an operand)
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(u), "+v"(w));
+    a = __builtin_bit_cast(float, u), b = __builtin_bit_cast(float, w);
+}
+__device__ __forceinline__ float max_both_halves(float x)
+{
+    float a, b;
+    both_halves(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_both_halves(float x)
+{
+    float a, b;
+    both_halves(x, a, b);
+    return a + b;
+}
 
 // 8 values of a result tile as an operand, rounded to the element type (to nearest even; fp32: kept)
 template <typename T>
@@ -63,14 +81,6 @@ __device__ __forceinline__ x8<T> as_operand(const f32x16 &w, int t)
     return r;
 }
 
-constexpr int pow2_at_least(int x)
-{
-    int p = 4;
-    while (p < x)
-        p *= 2;
-    return p;
-}
-
 // A tile of rows of DP = 32 DT features in LDS: 16-byte chunks, LC (a power of two) per row, chunk c of row r at place
 // c ^ swz(r).  swz is linear over the bits of r and chosen so that both ways of reading spread over the 64 banks: 16 rows
 // at one chunk (row_frag), and 4 consecutive rows at 4 consecutive chunks (col_frag of the 16-bit types).
@@ -79,8 +89,8 @@ struct Tile {
     static constexpr int ESZ = sizeof(T);
     static constexpr int EPC = 16 / ESZ;           // elements per chunk
     static constexpr int NCH = 32 * DT / EPC;      // chunks a row has
-    static constexpr int LC = pow2_at_least(NCH);  // places a row has
-    static constexpr int ROWB = LC * 16;
+    static constexpr int ROWB = attend_row_bytes(ESZ, DT);
+    static constexpr int LC = ROWB / 16;           // places a row has, a power of two
     static constexpr int KS = 2 * DT;              // matrix steps over the features
 
     static __device__ __host__ constexpr int swz(int r)
@@ -152,8 +162,8 @@ struct RowAt {
 __device__ __forceinline__ RowAt row_at(const AttendRows &rw, int bz, int hk, int r)
 {
     RowAt w;
-    const int n = r / rw.G, g = r - n * rw.G;
-    const int db = n / rw.M;
+    const int n = rw.by_g(r), g = r - n * rw.G;
+    const int db = rw.by_m(n);
     w.b = bz + db;
     w.i = n - db * rw.M;
     w.h = hk * rw.G + g;
