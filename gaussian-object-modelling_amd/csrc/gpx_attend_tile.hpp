@@ -235,7 +235,13 @@ __device__ __forceinline__ void dma4(u32x4 buffer, unsigned offset, unsigned lds
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// (the builtin tells the compiler that its own loads have arrived too: without it, fragments loaded before a loop are waited for at
+// their first use inside it, in every round, and with them the tile that was just asked for)
+__device__ __forceinline__ void dma_wait()
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+}
 __device__ __forceinline__ unsigned lds_offset(const void *p) { return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)p; }
 
 // how the 4 waves of a workgroup fill a tile of BN rows: instruction x of a wave takes the places from 64 (4 x + wave) on
