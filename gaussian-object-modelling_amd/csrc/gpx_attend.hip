@@ -121,7 +121,21 @@ void cut(int64_t blocks, int64_t n, int step, int least, int cus, int per_cu, in
 
 int64_t blocks_of(int64_t rows, int64_t per) { return (rows + per - 1) / per; }
 
+// Waves along the rows: the more rows share a tile of keys, the less often the keys are read -- as long as the workgroups, times the
+// pieces the key range may be cut into, give every CU one; else fewer rows and more of the key range at once.
+int waves_for(int esz, int dt, int64_t rows, int64_t groups, int64_t n, int (*step)(int esz, int dt, int wm), int least, int cus)
+{
+    const int lo = attend_least_wm(esz, dt);
+    int wm = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    while (wm > lo && blocks_of(rows, 32 * wm) * groups * std::max<int64_t>(1, n / step(esz, dt, wm) / least) < cus)
+        wm /= 2;
+    return std::max(wm, lo);
+}
+int fwd_step(int esz, int dt, int wm) { return attend_fwd_bn(esz, dt, wm); }
+int dq_step(int, int, int wm) { return attend_dq_bn(wm); }
+
 struct Plan {
+    int wm = 4;                         // waves along the rows
     int splits = 1, chunk = 0;          // forward / the shared context
     int own_splits = 0, own_chunk = 0;  // the own part
     int mtiles = 1, own_mtiles = 1, ktiles = 1;  // workgroups along the rows, along the keys (backward)
@@ -143,10 +157,10 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
     const size_t rid = (size_t)a.batch * a.nq * a.heads;
     if (which == GPX_ATTEND_SHARED) {
         const int R = (int)(a.batch * a.nq * G), Ro = (int)(a.nq * G);
-        const int wm = attend_wm(esz, dt, R), wo = attend_wm(esz, dt, 1);
+        const int wm = p.wm = waves_for(esz, dt, R, a.heads_kv, a.nk, fwd_step, 1, cus), wo = attend_least_wm(esz, dt);
         p.mtiles = (int)blocks_of(R, 32 * wm), p.own_mtiles = (int)blocks_of(Ro, 32 * wo);
         if (a.nk > 0)
-            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), 1, cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
+            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), 1, cus, attend_fwd_per_cu(esz, dt, wm, true), &p.splits, &p.chunk);
         else
             p.splits = 0;
         if (a.n_own > 0 || a.nk == 0)
@@ -157,11 +171,12 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
         p.total = p.po + slots * rid * a.dim * sizeof(float);
         return p;
     }
-    const int R = (int)(a.nq * G), wm = attend_wm(esz, dt, R);
+    const int R = (int)(a.nq * G);
+    const int wm = p.wm = waves_for(esz, dt, R, a.heads_kv * a.batch, a.nk, which == GPX_ATTEND_FORWARD ? fwd_step : dq_step, LEAST_STEPS, cus);
     p.mtiles = (int)blocks_of(R, 32 * wm);
     const int64_t blocks = p.mtiles * a.heads_kv * a.batch;
     if (which == GPX_ATTEND_FORWARD) {
-        cut(blocks, a.nk, attend_fwd_bn(esz, dt, wm), LEAST_STEPS, cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
+        cut(blocks, a.nk, attend_fwd_bn(esz, dt, wm), LEAST_STEPS, cus, attend_fwd_per_cu(esz, dt, wm, false), &p.splits, &p.chunk);
         if (p.splits > 1) {
             p.po = up(p.splits * rid * sizeof(float2));
             p.total = p.po + p.splits * rid * a.dim * sizeof(float);
@@ -212,9 +227,9 @@ AttendRows rows_of(const gpx_attend_args &a)
     r.by_hk = DivBy((unsigned)r.Hk);
     return r;
 }
-void set_grid(AttendFwd &f, int mtiles, int splits, int chunk)
+void set_grid(AttendFwd &f, int wm, int mtiles, int splits, int chunk)
 {
-    f.mtiles = mtiles, f.splits = splits, f.chunk = chunk;
+    f.wm = wm, f.mtiles = mtiles, f.splits = splits, f.chunk = chunk;
     f.by_mtiles = DivBy((unsigned)mtiles);
     f.by_splits = DivBy((unsigned)std::max(1, splits));
 }
@@ -290,7 +305,7 @@ extern "C" int gpx_attend(const gpx_attend_args *args)
     f.rows = rows_of(a);
     f.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
     f.c = (float)(a.scale * ATTEND_LOG2E);
-    set_grid(f, p.mtiles, p.splits, p.chunk);
+    set_grid(f, p.wm, p.mtiles, p.splits, p.chunk);
     f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
     f.lse = a.lse;
     f.slot_rows = (long)(a.batch * a.nq * a.heads);
@@ -331,11 +346,11 @@ extern "C" int gpx_attend_shared(const gpx_attend_args *args)
     w.first.rows.R = (int)(a.batch * a.nq) * w.first.rows.G;
     w.first.rows.grid_b = 1;
     w.first.keys = keys_of(a.k, a.v, a.nk, nullptr, nullptr, 0);
-    set_grid(w.first, p.mtiles, p.splits, p.chunk);
+    set_grid(w.first, p.wm, p.mtiles, p.splits, p.chunk);
     w.second.keys = keys_of(a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
     w.second.tail = 1;
     w.second.slot0 = p.splits;
-    set_grid(w.second, p.own_mtiles, p.own_splits, p.own_chunk);
+    set_grid(w.second, attend_least_wm(elem_size(a), attend_dt((int)a.dim)), p.own_mtiles, p.own_splits, p.own_chunk);
     return by_type(a, [&](auto t) {
         using T = decltype(t);
         attend_launch_pair<T>(w, (hipStream_t)a.stream);
@@ -364,7 +379,7 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.dout = a.d_o.p, b.gb = a.d_o.batch, b.gr = a.d_o.row, b.gh = a.d_o.head;
     b.lse = a.lse;
     b.stat = (float *)((char *)a.workspace + p.ml);
-    b.mtiles = p.mtiles, b.ktiles = p.ktiles;
+    b.wm = p.wm, b.mtiles = p.mtiles, b.ktiles = p.ktiles;
     b.by_mtiles = DivBy((unsigned)std::max(1, p.mtiles));
     b.by_ktiles = DivBy((unsigned)std::max(1, p.ktiles));
     b.by_q_splits = DivBy((unsigned)p.splits);

@@ -50,7 +50,7 @@ struct AttendFwd {
     float c = 0;            // scale log2(e): weights are 2^(c s - m)
     int tail = 0;           // 1: query i sees keys < len - (M - 1 - i)
     int splits = 1, chunk = 0;  // the key range in pieces of `chunk` rows, one workgroup each
-    int mtiles = 1;             // workgroups along the rows
+    int wm = 4, mtiles = 1;     // waves and workgroups along the rows
     DivBy by_mtiles, by_splits;
     void *o = nullptr;      // splits == 1 and po == null
     long ob = 0, orow = 0, oh = 0;
@@ -92,6 +92,7 @@ struct AttendBwd {
     void *dq = nullptr, *dk = nullptr, *dv = nullptr;
     long dqb = 0, dqr = 0, dqh = 0, dkb = 0, dkr = 0, dkh = 0, dvb = 0, dvr = 0, dvh = 0;
     int q_splits = 1, q_chunk = 0;   // dQ: pieces of the key range
+    int wm = 4;                      // dQ: waves along the rows
     int mtiles = 1, ktiles = 1;      // workgroups along the rows (dQ) and along the keys (dK, dV)
     DivBy by_mtiles, by_ktiles, by_q_splits, by_k_splits;
     int k_splits = 1, k_chunk = 0;   // dK, dV: pieces of the row range
@@ -108,17 +109,17 @@ constexpr int attend_row_bytes(int esz, int dt)  // of a row in LDS: a power of 
         p *= 2;
     return p;
 }
-// Waves along the rows (32 packed rows each); what is left of a workgroup's 4 waves takes parts of the key range.  (fp32 rows of
-// more than 64 features: two at least, four waves' tiles of keys would not fit.)
-constexpr int attend_wm(int esz, int dt, int rows) { return rows <= 32 && !(esz == 4 && dt > 2) ? 1 : rows <= 64 ? 2 : 4; }
+// Waves along the rows (32 packed rows each): 1, 2 or 4; what is left of a workgroup's 4 waves takes parts of the key range.  (fp32
+// rows of more than 64 features: two at least, four waves' tiles of keys would not fit.)
+constexpr int attend_least_wm(int esz, int dt) { return esz == 4 && dt > 2 ? 2 : 1; }
 constexpr int attend_fwd_kt(int esz, int dt, int wm) { return esz == 2 && wm == 4 ? 64 : 32; }  // keys of a wave per step
 constexpr int attend_fwd_bn(int esz, int dt, int wm) { return attend_fwd_kt(esz, dt, wm) * (4 / wm); }
 constexpr int attend_fwd_lds(int esz, int dt, int wm, int stages) { return stages * 2 * attend_fwd_bn(esz, dt, wm) * attend_row_bytes(esz, dt); }
 constexpr int attend_lds_per_cu(int bytes) { return bytes <= 38 * 1024 ? 4 : bytes <= 52 * 1024 ? 3 : bytes <= 78 * 1024 ? 2 : 1; }
 // workgroups a CU holds: LDS, and the registers of a wave (512 a SIMD lane, so waves per SIMD = workgroups per CU)
-constexpr int attend_fwd_per_cu(int esz, int dt, int wm)
+constexpr int attend_fwd_per_cu(int esz, int dt, int wm, bool pair)
 {
-    const int regs = dt == 4 || (esz == 4 && dt == 3) ? 2 : dt == 3 ? 2 : esz == 4 && dt == 2 ? 2 : 3;
+    const int regs = esz == 4 ? (dt == 1 ? 3 : dt <= 2 + !pair ? 2 : 1) : dt <= 2 ? 3 : 2;
     const int lds = attend_lds_per_cu(attend_fwd_lds(esz, dt, wm, 2));
     return lds < regs ? lds : regs;
 }

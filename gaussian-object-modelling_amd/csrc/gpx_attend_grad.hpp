@@ -90,13 +90,13 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
         look(begin + BN);
     }
 
-    x8<T> qf[2 * DT], gf[2 * DT];
+    Frag<T> qf[2 * DT], gf[2 * DT];
     load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
     load_row_frags<T, DT>(gf, (const T *)a.dout + (at.valid ? at.b * a.gb + at.i * a.gr + at.h * a.gh : 0), at.valid, rw.D, lane);
     // lse in log2 units (+inf where the row has no weights, so that every p is 0), and <dO, O>
     float lse = POS_INF, dd = 0.0f;
     {
-        x8<T> of[2 * DT];
+        Frag<T> of[2 * DT];
         load_row_frags<T, DT>(of, (const T *)a.o + (at.valid ? at.b * a.ob + at.i * a.orow + at.h * a.oh : 0), at.valid, rw.D, lane);
         const long rid = ((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i;
         const float from = at.valid ? a.lse[rid] : NEG_INF;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
         for (int t = 0; t < 2 * DT; ++t)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                dd += (float)gf[t][j] * (float)of[t][j];
+                dd += gf[t][j] * of[t][j];
         dd = sum_both_halves(dd);
         if (from != NEG_INF)
             lse = from * 1.44269504088896f;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
             sc[i] = exp2_(sc[i] * a.c - lse) * (dp[i] - dd);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const x8<T> ds = as_operand<T>(sc, t);
+            const Frag<T> ds = as_operand<T>(sc, t);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 dq[d] = mma(TL::col_frag(kt, cbase, wk * KT + 16 * t, d), ds, dq[d]);
@@ -197,34 +197,13 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
                     dq[d][i] += w[(d * 16 + i) * 64 + lane];
         }
     }
-    if (!at.exists)
-        return;
     if (a.pq) {
         const long rid = ((long)at.b * rw.M + at.i) * ((long)rw.Hk * rw.G) + at.h;
         float *p = a.pq + ((long)split * ((long)rw.grid_b * rw.M * rw.Hk * rw.G) + rid) * rw.D;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int f = 32 * d + 8 * x + 4 * half;
-                if (f < rw.D)
-                    *reinterpret_cast<f32x4 *>(p + f) = f32x4{dq[d][4 * x], dq[d][4 * x + 1], dq[d][4 * x + 2], dq[d][4 * x + 3]};
-            }
+        store_column<float, DT>(p, dq, rw.D, half, at.exists, [](float x) { return x; });
         return;
     }
-    T *p = (T *)a.dq + at.b * a.dqb + at.i * a.dqr + at.h * a.dqh;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int f = 32 * d + 8 * x + 4 * half;
-            x4<T> w;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[k] = (T)(dq[d][4 * x + k] * a.scale);
-            if (f < rw.D)
-                *reinterpret_cast<x4<T> *>(p + f) = w;
-        }
+    store_column<T, DT>((T *)a.dq + at.b * a.dqb + at.i * a.dqr + at.h * a.dqh, dq, rw.D, half, at.exists, [&](float x) { return x * a.scale; });
 }
 
 // dK, dV: 4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one
@@ -290,7 +269,7 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
     if (begin < end)
         fetch(begin, 0);
 
-    x8<T> kf[2 * DT], vf[2 * DT];
+    Frag<T> kf[2 * DT], vf[2 * DT];
     {
         const int lane = lane_again(), key = key0 + (lane & 31);
         const bool counts = counts_of(key);
@@ -338,14 +317,14 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const x8<T> w = as_operand<T>(p, t);
+                const Frag<T> w = as_operand<T>(p, t);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
                     dv[d] = mma(TL::col_frag(gt, cbase, 16 * t, d), w, dv[d]);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const x8<T> w = as_operand<T>(dp, t);
+                const Frag<T> w = as_operand<T>(dp, t);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
                     dk[d] = mma(TL::col_frag(qt, cbase, 16 * t, d), w, dk[d]);
@@ -353,49 +332,24 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
         }
     }
     const int lane = lane_again(), half = lane >> 5, key = key0 + (lane & 31);
-    if (key >= a.keys.n)
-        return;
-    const bool counts = counts_of(key);
-    // a key that does not count had zeros for its fragments: its sums are of finite weights but not zero
-    const float fk = counts ? 1.0f : 0.0f;
-    if (a.pk) {
-        const long at = ((long)split * rw.grid_b * rw.Hk + (long)bz * rw.Hk + hk) * a.keys.n + key;
-        float *pk = a.pk + at * rw.D, *pv = a.pv + at * rw.D;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int f = 32 * d + 8 * x + 4 * half;
-                f32x4 wk, wv;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    wk[j] = fk == 0.0f ? 0.0f : dk[d][4 * x + j];
-                    wv[j] = fk == 0.0f ? 0.0f : dv[d][4 * x + j];
-                }
-                if (f < rw.D) {
-                    *reinterpret_cast<f32x4 *>(pk + f) = wk;
-                    *reinterpret_cast<f32x4 *>(pv + f) = wv;
-                }
-            }
-        return;
-    }
-    T *pk = (T *)a.dk + bz * a.dkb + key * a.dkr + hk * a.dkh, *pv = (T *)a.dv + bz * a.dvb + key * a.dvr + hk * a.dvh;
+    const bool exists = key < a.keys.n, counts = exists && counts_of(key);
+    // a key that does not count had zeros for its features: its sums are of finite weights but not zero
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int f = 32 * d + 8 * x + 4 * half;
-            x4<T> wk, wv;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                wk[j] = fk == 0.0f ? (T)0.0f : (T)(dk[d][4 * x + j] * a.scale);
-                wv[j] = fk == 0.0f ? (T)0.0f : (T)dv[d][4 * x + j];
-            }
-            if (f < rw.D) {
-                *reinterpret_cast<x4<T> *>(pk + f) = wk;
-                *reinterpret_cast<x4<T> *>(pv + f) = wv;
-            }
+        for (int i = 0; i < 16; ++i) {
+            dk[d][i] = counts ? dk[d][i] : 0.0f;
+            dv[d][i] = counts ? dv[d][i] : 0.0f;
         }
+    const auto same = [](float x) { return x; };
+    if (a.pk) {
+        const long at = ((long)split * rw.grid_b * rw.Hk + (long)bz * rw.Hk + hk) * a.keys.n + key;
+        store_column<float, DT>(a.pk + at * rw.D, dk, rw.D, half, exists, same);
+        store_column<float, DT>(a.pv + at * rw.D, dv, rw.D, half, exists, same);
+        return;
+    }
+    store_column<T, DT>((T *)a.dk + bz * a.dkb + key * a.dkr + hk * a.dkh, dk, rw.D, half, exists, [&](float x) { return x * a.scale; });
+    store_column<T, DT>((T *)a.dv + bz * a.dvb + key * a.dvr + hk * a.dvh, dv, rw.D, half, exists, same);
 }
 
 // out[row] = f sum_s p[s][row], in slot order; rows of D values, four per lane.  Row -> (batch, n, head) by the strides.  Up to
@@ -455,9 +409,9 @@ void launch_bwd_dim(const AttendBwd &a, hipStream_t st)
     const dim3 block(256);
     if (a.rows.R > 0) {
         const dim3 grid((unsigned)(a.mtiles * a.q_splits * a.rows.Hk * a.rows.grid_b));
-        switch (attend_wm(sizeof(T), DT, a.rows.R)) {
+        switch (a.wm) {
         case 1:
-            if constexpr (attend_wm(sizeof(T), DT, 1) == 1)
+            if constexpr (attend_least_wm(sizeof(T), DT) == 1)
                 hipLaunchKernelGGL((attend_dq_kernel<T, DT, 1>), grid, block, 0, st, a);
             break;
         case 2: hipLaunchKernelGGL((attend_dq_kernel<T, DT, 2>), grid, block, 0, st, a); break;

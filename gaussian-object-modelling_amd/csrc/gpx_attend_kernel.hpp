@@ -90,7 +90,7 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
         look(begin + BN);
     }
 
-    x8<T> qf[2 * DT];
+    Frag<T> qf[2 * DT];
     load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
 
     f32x16 o[DT];
@@ -173,7 +173,7 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const x8<T> p = as_operand<T>(sc[s], t);
+                const Frag<T> p = as_operand<T>(sc[s], t);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
                     o[d] = mma(TL::col_frag(vt, cbase, wk * KT + 32 * s + 16 * t, d), p, o[d]);
@@ -237,49 +237,27 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
                     o[d][i] = o[d][i] * f0 + w[(d * 16 + i) * 64 + lane] * f1;
         }
     }
-    if (!at.exists)
-        return;
     const long rid = ((long)at.b * rw.M + at.i) * ((long)rw.Hk * rw.G) + at.h;
     if (!at.valid)
         m = NEG_INF, l = 0.0f;
     if (a.po) {
         const long slot = (long)(a.slot0 + split) * a.slot_rows + rid;
-        if (half == 0)
+        if (half == 0 && at.exists)
             a.pml[slot] = make_float2(m, l);
-        if (l == 0.0f)
-            return;  // a piece without weights is never read
-        float *po = a.po + slot * rw.D;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int f = 32 * d + 8 * x + 4 * half;
-                if (f < rw.D)
-                    *reinterpret_cast<f32x4 *>(po + f) = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
-            }
+        // (a piece without weights is never read)
+        store_column<float, DT>(a.po + slot * rw.D, o, rw.D, half, at.exists && l != 0.0f, [](float x) { return x; });
         return;
     }
-    if (half == 0)
-        a.lse[((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i] = l == 0.0f ? NEG_INF : (m + log2_(l)) * 0.693147180559945f;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const bool none = l == 0.0f;
-    T *po = (T *)a.o + at.b * a.ob + at.i * a.orow + at.h * a.oh;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int f = 32 * d + 8 * x + 4 * half;
-            x4<T> w;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = none ? (T)0.0f : (T)(o[d][4 * x + j] * inv);
-            if (f < rw.D)
-                *reinterpret_cast<x4<T> *>(po + f) = w;
-        }
+    if (half == 0 && at.exists)
+        a.lse[((long)at.b * rw.Hk * rw.G + at.h) * rw.M + at.i] = none ? NEG_INF : (m + log2_(l)) * 0.693147180559945f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    store_column<T, DT>((T *)a.o + at.b * a.ob + at.i * a.orow + at.h * a.oh, o, rw.D, half, at.exists,
+                        [=](float x) { return none ? 0.0f : x * inv; });
 }
 
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_fwd_kernel(AttendFwd a)
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, false))) void attend_fwd_kernel(AttendFwd a)
 {
     __shared__ __attribute__((aligned(1024))) char lds[attend_fwd_lds(sizeof(T), DT, WM, 2)];
     __shared__ __attribute__((aligned(16))) float bias[2 * attend_fwd_bn(sizeof(T), DT, WM)];
@@ -288,9 +266,9 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void a
 
 // Both parts of a shared call in one launch.  The own part has few rows per workgroup whatever the first has.
 template <typename T, int DT>
-constexpr int own_wm() { return attend_wm(sizeof(T), DT, 1); }
+constexpr int own_wm() { return attend_least_wm(sizeof(T), DT); }
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_pair_kernel(AttendPair a)
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, true))) void attend_pair_kernel(AttendPair a)
 {
     constexpr int OWN = own_wm<T, DT>();
     constexpr int A = attend_fwd_lds(sizeof(T), DT, WM, 2), B = attend_fwd_lds(sizeof(T), DT, OWN, 1);
@@ -377,7 +355,7 @@ template <typename T, int DT>
 void launch_fwd_dim(const AttendFwd &a, hipStream_t st)
 {
     const dim3 grid((unsigned)a.blocks()), block(256);
-    switch (attend_wm(sizeof(T), DT, a.rows.R)) {
+    switch (a.wm) {
     case 1:
         if constexpr (own_wm<T, DT>() == 1)
             hipLaunchKernelGGL((attend_fwd_kernel<T, DT, 1>), grid, block, 0, st, a);
@@ -390,7 +368,7 @@ template <typename T, int DT>
 void launch_pair_dim(const AttendPair &a, hipStream_t st)
 {
     const dim3 grid((unsigned)(a.first.blocks() + a.second.blocks())), block(256);
-    switch (attend_wm(sizeof(T), DT, a.first.rows.R)) {
+    switch (a.first.wm) {
     case 1:
         if constexpr (own_wm<T, DT>() == 1)
             hipLaunchKernelGGL((attend_pair_kernel<T, DT, 1>), grid, block, 0, st, a);

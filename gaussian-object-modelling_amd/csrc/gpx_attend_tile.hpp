@@ -2,8 +2,9 @@
 //
 // Everything is built from one 32 x 32 matrix step with 16 terms of the sum.  Its operand of a lane is 8 values: row (or column)
 // lane % 32, terms 8 (lane / 32) .. + 7; its result is 16 values: column lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4.
-// 16-bit types: one v_mfma_f32_32x32x16; fp32: eight v_mfma_f32_32x32x2 over the same 8 values (the order of the terms does
-// not matter as long as both operands agree on it).
+// 16-bit types: one v_mfma_f32_32x32x16.  fp32: each value is cut into three bf16 pieces of 8 bits, exactly (24 bits in all), and
+// of the nine products of pieces the six that reach 2^-24 of the result are summed in fp32, smallest first: the accuracy of a
+// chain of fp32 products at 6 x 32 cycles a step, where v_mfma_f32_32x32x2_f32 takes 8 x 64 (measured: see below).
 //
 // That freedom is used once more: a result tile W (rows = terms of the NEXT product) goes into it as an operand without
 // leaving its lane -- registers 8 t .. 8 t + 7 are the terms { 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4 } -- and the other
@@ -35,14 +36,56 @@ template <> struct Elem<__bf16> {
 template <typename T> using x8 = typename Elem<T>::x8;
 template <typename T> using x4 = typename Elem<T>::x4;
 
-__device__ __forceinline__ f32x16 mma(x8<_Float16> a, x8<_Float16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(x8<__bf16> a, x8<__bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(x8<float> a, x8<float> b, f32x16 c)
-{
+// A lane's 8 values of an operand, as the matrix cores take them.
+template <typename T>
+struct Frag {
+    x8<T> v;
+    __device__ __forceinline__ static Frag of(x8<T> x) { return {x}; }
+    __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
+};
+template <>
+struct Frag<float> {
+    x8<__bf16> h, m, l;  // the upper, middle and lower 8 bits of each value; their sum is the value
+    __device__ __forceinline__ static Frag of(x8<float> x)
+    {
+        u32x4 h, m, l;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
+        for (int j = 0; j < 4; ++j) {
+            unsigned a[3], b[3];
+            cut(x[2 * j], a);
+            cut(x[2 * j + 1], b);
+            h[j] = __builtin_amdgcn_perm(b[0], a[0], 0x07060302);  // the upper halves of two values
+            m[j] = __builtin_amdgcn_perm(b[1], a[1], 0x07060302);
+            l[j] = __builtin_amdgcn_perm(b[2], a[2], 0x07060302);
+        }
+        return {__builtin_bit_cast(x8<__bf16>, h), __builtin_bit_cast(x8<__bf16>, m), __builtin_bit_cast(x8<__bf16>, l)};
+    }
+    __device__ __forceinline__ static void cut(float x, unsigned (&p)[3])  // pieces in the upper halves
+    {
+        p[0] = __builtin_bit_cast(unsigned, x);
+        const float r = x - __builtin_bit_cast(float, p[0] & 0xffff0000u);
+        p[1] = __builtin_bit_cast(unsigned, r);
+        const float s = r - __builtin_bit_cast(float, p[1] & 0xffff0000u);
+        p[2] = __builtin_bit_cast(unsigned, s);
+    }
+    __device__ __forceinline__ float operator[](int j) const { return ((float)l[j] + (float)m[j]) + (float)h[j]; }
+};
+
+__device__ __forceinline__ f32x16 mma16(x8<_Float16> a, x8<_Float16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma16(x8<__bf16> a, x8<__bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <typename T>
+__device__ __forceinline__ f32x16 mma(const Frag<T> &a, const Frag<T> &b, f32x16 c)
+{
+    if constexpr (sizeof(T) == 2) {
+        return mma16(a.v, b.v, c);
+    } else {
+        c = mma16(a.l, b.h, c);
+        c = mma16(a.h, b.l, c);
+        c = mma16(a.m, b.m, c);
+        c = mma16(a.m, b.h, c);
+        c = mma16(a.h, b.m, c);
+        return mma16(a.h, b.h, c);
+    }
 }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32, 1 ulp
@@ -72,13 +115,13 @@ __device__ __forceinline__ float sum_both_halves(float x)
 
 // 8 values of a result tile as an operand, rounded to the element type (to nearest even; fp32: kept)
 template <typename T>
-__device__ __forceinline__ x8<T> as_operand(const f32x16 &w, int t)
+__device__ __forceinline__ Frag<T> as_operand(const f32x16 &w, int t)
 {
     x8<T> r;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         r[j] = (T)w[8 * t + j];
-    return r;
+    return Frag<T>::of(r);
 }
 
 // A tile of rows of DP = 32 DT features in LDS: 16-byte chunks, LC (a power of two) per row, chunk c of row r at place
@@ -107,14 +150,14 @@ struct Tile {
         return r * ROWB + ((c ^ swz(r)) << 4);
     }
     // rows row0 .. row0 + 31 (row0: a multiple of 32), features 16 t .. 16 t + 15
-    static __device__ __forceinline__ x8<T> row_frag(const char *tile, int base, int row0, int t)
+    static __device__ __forceinline__ Frag<T> row_frag(const char *tile, int base, int row0, int t)
     {
         if constexpr (ESZ == 2) {
-            return __builtin_bit_cast(x8<T>, *reinterpret_cast<const u32x4 *>(tile + row0 * ROWB + (base ^ (t << 5))));
+            return Frag<T>::of(__builtin_bit_cast(x8<T>, *reinterpret_cast<const u32x4 *>(tile + row0 * ROWB + (base ^ (t << 5)))));
         } else {
             const f32x4 lo = *reinterpret_cast<const f32x4 *>(tile + row0 * ROWB + (base ^ (t << 6)));
             const f32x4 hi = *reinterpret_cast<const f32x4 *>(tile + row0 * ROWB + (base ^ (t << 6) ^ 16));
-            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return Frag<T>::of(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
     // lane part of col_frag's address.  16-bit: ds_read_b64_tr_b16 takes from each lane of a block of 16 the address of 4
@@ -132,7 +175,7 @@ struct Tile {
         }
     }
     // column 32 dt + lane % 32 of the rows row0 + { 8 (j / 4) + 4 (lane / 32) + j % 4 }, j = 0 .. 7 (row0: a multiple of 16)
-    static __device__ __forceinline__ x8<T> col_frag(const char *tile, int base, int row0, int dt)
+    static __device__ __forceinline__ Frag<T> col_frag(const char *tile, int base, int row0, int dt)
     {
         if constexpr (ESZ == 2) {
             typedef __attribute__((address_space(3))) s16x4 *lds4;
@@ -140,7 +183,7 @@ struct Tile {
             const char *p1 = tile + (row0 + 8) * ROWB + (base ^ (dt << 6) ^ (swz(8) << 4));
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p0);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p1);
-            return __builtin_bit_cast(x8<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            return Frag<T>::of(__builtin_bit_cast(x8<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)));
         } else {
             x8<T> r;
 #pragma unroll
@@ -148,7 +191,7 @@ struct Tile {
                 const int k = 8 * (j >> 2) + (j & 3);
                 r[j] = *reinterpret_cast<const float *>(tile + (row0 + k) * ROWB + (base ^ (dt << 7) ^ (swz(k) << 4)));
             }
-            return r;
+            return Frag<T>::of(r);
         }
     }
 };
@@ -176,7 +219,7 @@ __device__ __forceinline__ RowAt row_at(const AttendRows &rw, int bz, int hk, in
 
 // operand fragments of one row per lane straight from memory (zero where the row does not count or the feature is padding)
 template <typename T, int DT>
-__device__ __forceinline__ void load_row_frags(x8<T> (&f)[2 * DT], const T *p, bool valid, int D, int lane)
+__device__ __forceinline__ void load_row_frags(Frag<T> (&f)[2 * DT], const T *p, bool valid, int D, int lane)
 {
     const int h = lane >> 5;
 #pragma unroll
@@ -186,9 +229,9 @@ __device__ __forceinline__ void load_row_frags(x8<T> (&f)[2 * DT], const T *p, b
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             z[j] = (T)0.0f;
-        f[t] = z;
         if (valid && d < D)
-            f[t] = *reinterpret_cast<const x8<T> *>(p + d);
+            z = *reinterpret_cast<const x8<T> *>(p + d);
+        f[t] = Frag<T>::of(z);
     }
 }
 
@@ -263,6 +306,46 @@ struct Fill {
     }
     static __device__ __forceinline__ unsigned lds(int x, int wave) { return 1024u * (4 * x + wave); }
 };
+
+// A lane's column of a result of DT tiles (rows = features) to memory, rounded once: f(value) -> value to store.  A lane holds 4
+// consecutive features at a time, the other half of the wave the next 4; the 16-bit types swap pieces between the halves first,
+// so that every store is 16 bytes.  Features from D on are padding.
+template <typename T, int DT, typename F>
+__device__ __forceinline__ void store_column(T *p, const f32x16 (&r)[DT], int D, int half, bool on, F f)
+{
+    if constexpr (sizeof(T) == 4) {
+        if (!on)
+            return;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int at = 32 * d + 8 * x + 4 * half;
+                if (at < D)
+                    *reinterpret_cast<f32x4 *>(p + at) = f32x4{f(r[d][4 * x]), f(r[d][4 * x + 1]), f(r[d][4 * x + 2]), f(r[d][4 * x + 3])};
+            }
+    } else {
+        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; x += 2) {
+                x4<T> a, b;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[j] = (T)f(r[d][4 * x + j]);
+                    b[j] = (T)f(r[d][4 * x + 4 + j]);
+                }
+                u32x2 ua = __builtin_bit_cast(u32x2, a), ub = __builtin_bit_cast(u32x2, b);
+                unsigned a0 = ua[0], a1 = ua[1], b0 = ub[0], b1 = ub[1];
+                // the upper lanes' a for the lower lanes' b: then a lane has 8 features in a row, of piece x or x + 1
+                asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %2\n\tv_permlane32_swap_b32 %1, %3" : "+v"(a0), "+v"(a1), "+v"(b0), "+v"(b1));
+                const int at = 32 * d + 8 * (x + half);
+                if (on && at < D)
+                    *reinterpret_cast<u32x4 *>(p + at) = u32x4{a0, a1, b0, b1};
+            }
+    }
+}
 
 // weights of masked places: register i of a result tile is row 8 (i / 4) + 4 half + i % 4
 __device__ __forceinline__ bool bit_of(unsigned m, int half, int i) { return (m >> (8 * (i >> 2) + 4 * half + (i & 3))) & 1u; }
