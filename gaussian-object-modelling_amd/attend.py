@@ -23,6 +23,7 @@ _ARGS = struct.Struct("@iiqqqqqqqd" + "Pqqq" * 4 + "PPPPq" + "Pqqq" * 6 + "PPQP"
 _NONE = (0, 0, 0, 0)
 
 _calls = None
+_workspace = {}  # bytes gpx_attend_workspace gave for (call, scalar, device, sizes, scale)
 
 
 def _entry(which):
@@ -78,10 +79,11 @@ def _operand(x, name, q, shape, group=1):
     return x, (p, b, r, h)
 
 
-def _like(shape, q):
-    x = torch.empty(shape, dtype=q.dtype, device=q.device)
-    b, r, h, _ = x.stride()
-    return x, (x.data_ptr(), b, r, h)
+def _like(x):
+    """A contiguous tensor of x's shape, and its gpx_view."""
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r, h, d = x.shape[1:]
+    return y, (y.data_ptr(), r * h * d, h * d, d)
 
 
 def _lengths(x, name, q):
@@ -109,13 +111,18 @@ def _run(which, q, rest):
     index = q.device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
     head = (_SCALARS[q.dtype], index) + rest
-    args = _ARGS.pack(*head, 0, 0, stream)
-    need = C.c_size_t(0)
-    _check(_entry(3)(args, which, C.byref(need)))
-    if need.value:
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        args = _ARGS.pack(*head, work.data_ptr(), need.value, stream)
-    _check(_entry(which)(args))
+    sizes = (which,) + head[:10]
+    need = _workspace.get(sizes)
+    if need is None:
+        n = C.c_size_t(0)
+        _check(_entry(3)(_ARGS.pack(*head, 0, 0, stream), which, C.byref(n)))
+        if len(_workspace) >= 4096:
+            _workspace.clear()
+        need = _workspace[sizes] = n.value
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = _entry(which)(_ARGS.pack(*head, work.data_ptr() if need else 0, need, stream))
+    if rc:
+        _check(rc)
 
 
 def attend(q, k, v, scale=None, k_len=None, key_mask=None, q_len=None):
@@ -128,7 +135,7 @@ def attend(q, k, v, scale=None, k_len=None, key_mask=None, q_len=None):
     q, qv = _operand(q, "q", q, q.shape, hq // hk)
     k, kv = _operand(k, "k", q, (b, nk, hk, d))
     v, vv = _operand(v, "v", q, (b, nk, hk, d))
-    o, ov = _like((b, nq, hq, d), q)
+    o, ov = _like(q)
     lse = torch.empty((b, hq, nq), dtype=torch.float32, device=q.device)
     _run(FORWARD, q, (b, nq, nk, 0, hq, hk, d, scale) + qv + kv + vv + ov
          + (lse.data_ptr(), _lengths(q_len, "q_len", q), _lengths(k_len, "k_len", q)) + _mask(key_mask, q, nk) + _NONE * 6 + (0,))
@@ -149,9 +156,9 @@ def attend_backward(d_o, q, k, v, o, lse, scale=None, k_len=None, key_mask=None,
         _bad("lse must be a contiguous float32 tensor on the device of q")
     if lse.shape != (b, hq, nq):
         _bad("lse must be of shape %s, not %s" % ([b, hq, nq], list(lse.shape)), E_SIZE_MISMATCH)
-    dq, dqv = _like((b, nq, hq, d), q)
-    dk, dkv = _like((b, nk, hk, d), q)
-    dv, dvv = _like((b, nk, hk, d), q)
+    dq, dqv = _like(q)
+    dk, dkv = _like(k)
+    dv, dvv = _like(v)
     _run(BACKWARD, q, (b, nq, nk, 0, hq, hk, d, scale) + qv + kv + vv + ov
          + (lse.data_ptr(), _lengths(q_len, "q_len", q), _lengths(k_len, "k_len", q)) + _mask(key_mask, q, nk)
          + gv + dqv + dkv + dvv + _NONE * 2 + (0,))
@@ -172,7 +179,7 @@ def attend_shared(q, k, v, k_own, v_own, own_len=None, scale=None):
     v, vv = _operand(v[None], "v", q, (1, nk, hk, d))
     k_own, kov = _operand(k_own, "k_own", q, (b, no, hk, d))
     v_own, vov = _operand(v_own, "v_own", q, (b, no, hk, d))
-    o, ov = _like((b, nq, hq, d), q)
+    o, ov = _like(q)
     lse = torch.empty((b, hq, nq), dtype=torch.float32, device=q.device)
     _run(SHARED, q, (b, nq, nk, no, hq, hk, d, scale) + qv + kv + vv + ov + (lse.data_ptr(), 0, 0, 0, 0) + _NONE * 4 + kov + vov
          + (_lengths(own_len, "own_len", q),))

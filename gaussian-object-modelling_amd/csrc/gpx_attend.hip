@@ -16,11 +16,12 @@ struct DeviceScope {  // the call runs on args->device; the caller's current dev
     }
     int enter(int dev)
     {
-        if (dev < 0)
-            return GPX_OK;
         int cur = -1;
-        HIPCHK(hipGetDevice(&cur));
-        if (cur == dev)
+        if (hipGetDevice(&cur) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail(GPX_E_NO_DEVICE, "no HIP device: libgpx has no CPU path");
+        }
+        if (dev < 0 || cur == dev)
             return GPX_OK;
         HIPCHK(hipSetDevice(dev));
         before = cur;
@@ -160,7 +161,8 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
         const int wm = p.wm = waves_for(esz, dt, R, a.heads_kv, a.nk, fwd_step, 1, cus), wo = attend_least_wm(esz, dt);
         p.mtiles = (int)blocks_of(R, 32 * wm), p.own_mtiles = (int)blocks_of(Ro, 32 * wo);
         if (a.nk > 0)
-            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), 1, cus, attend_fwd_per_cu(esz, dt, wm, true), &p.splits, &p.chunk);
+            // a piece writes 4 bytes a row and feature where its keys are 2 esz: pieces of wm steps keep that below what they read
+            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), wm, cus, attend_fwd_per_cu(esz, dt, wm, true), &p.splits, &p.chunk);
         else
             p.splits = 0;
         if (a.n_own > 0 || a.nk == 0)
@@ -232,6 +234,7 @@ void set_grid(AttendFwd &f, int wm, int mtiles, int splits, int chunk)
     f.wm = wm, f.mtiles = mtiles, f.splits = splits, f.chunk = chunk;
     f.by_mtiles = DivBy((unsigned)mtiles);
     f.by_splits = DivBy((unsigned)std::max(1, splits));
+    f.order = attend_order(mtiles, (long)splits * f.rows.Hk * f.rows.grid_b, f.keys.len || f.rows.len);
 }
 AttendKeys keys_of(const gpx_view &k, const gpx_view &v, int64_t n, const int32_t *len, const uint8_t *mask, int64_t mask_b)
 {
@@ -267,8 +270,6 @@ int begin(const gpx_attend_args *pa, int which, DeviceScope &scope, Plan *plan)
         rc = check_data(*pa, which);
     if (rc != GPX_OK)
         return rc;
-    if (gpx_device_count() < 1)
-        return fail(GPX_E_NO_DEVICE, "no HIP device: libgpx has no CPU path");
     rc = scope.enter(pa->device);
     if (rc != GPX_OK)
         return rc;
@@ -382,6 +383,8 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.wm = p.wm, b.mtiles = p.mtiles, b.ktiles = p.ktiles;
     b.by_mtiles = DivBy((unsigned)std::max(1, p.mtiles));
     b.by_ktiles = DivBy((unsigned)std::max(1, p.ktiles));
+    b.q_order = attend_order(p.mtiles, (long)p.splits * b.rows.Hk * b.rows.grid_b, a.k_len || a.q_len);
+    b.k_order = attend_order(p.ktiles, (long)p.k_splits * b.rows.Hk * b.rows.grid_b, a.k_len || a.q_len);
     b.by_q_splits = DivBy((unsigned)p.splits);
     b.by_k_splits = DivBy((unsigned)p.k_splits);
     b.dq = a.dq.p, b.dqb = a.dq.batch, b.dqr = a.dq.row, b.dqh = a.dq.head;

@@ -44,6 +44,13 @@ struct AttendRows {
     DivBy by_m, by_g, by_hk;
 };
 
+// which workgroups share an XCD (gpx_attend_tile.hpp, place_block); whole groups need a multiple of 8 of them
+enum { ATTEND_WHOLE_GROUPS = 0, ATTEND_PIECES = 1, ATTEND_SPREAD = 2 };
+inline int attend_order(int tiles, long groups, bool ragged)
+{
+    return tiles > 1 && groups % 8 == 0 ? ATTEND_WHOLE_GROUPS : tiles > 1 && ragged ? ATTEND_SPREAD : ATTEND_PIECES;
+}
+
 struct AttendFwd {
     AttendRows rows;
     AttendKeys keys;
@@ -52,6 +59,7 @@ struct AttendFwd {
     int splits = 1, chunk = 0;  // the key range in pieces of `chunk` rows, one workgroup each
     int wm = 4, mtiles = 1;     // waves and workgroups along the rows
     DivBy by_mtiles, by_splits;
+    int order = 0;
     void *o = nullptr;      // splits == 1 and po == null
     long ob = 0, orow = 0, oh = 0;
     float *lse = nullptr;   // [B][H][M]
@@ -95,6 +103,7 @@ struct AttendBwd {
     int wm = 4;                      // dQ: waves along the rows
     int mtiles = 1, ktiles = 1;      // workgroups along the rows (dQ) and along the keys (dK, dV)
     DivBy by_mtiles, by_ktiles, by_q_splits, by_k_splits;
+    int q_order = 0, k_order = 0;
     int k_splits = 1, k_chunk = 0;   // dK, dV: pieces of the row range
     float *pq = nullptr;             // q_splits > 1: partial dQ [split][rid][D]
     float *pk = nullptr, *pv = nullptr;  // k_splits > 1: [split][(b Hk + hk) n + j][D]

@@ -27,8 +27,8 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
-    const unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int u = a.by_mtiles(id), mt = id - u * a.mtiles;
+    int mt, u;
+    place_block(blockIdx.x, gridDim.x, a.q_order, a.mtiles, a.by_mtiles, mt, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
     const int bz = a.by_q_splits(us), split = us - bz * a.q_splits;
 
@@ -226,8 +226,8 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
         return x;
     };
     const AttendRows &rw = a.rows;
-    const unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int u = a.by_ktiles(id), ktile = id - u * a.ktiles;
+    int ktile, u;
+    place_block(blockIdx.x, gridDim.x, a.k_order, a.ktiles, a.by_ktiles, ktile, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
     const int bz = a.by_k_splits(us), split = us - bz * a.k_splits;
 

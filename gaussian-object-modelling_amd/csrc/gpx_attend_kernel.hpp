@@ -16,7 +16,7 @@ namespace attend {
 // next is on its way.
 // STAGES == 1 has one tile at a time (the own part of a shared call: short ranges, many workgroups a CU).
 template <typename T, int DT, int WM, int STAGES>
-__device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, float *bias, unsigned id)
+__device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, float *bias, unsigned id, unsigned total)
 {
     using TL = Tile<T, DT>;
     constexpr int WK = 4 / WM, KT = attend_fwd_kt(sizeof(T), DT, WM), NS = KT / 32, BN = KT * WK;
@@ -26,7 +26,8 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
-    const int u = a.by_mtiles(id), mt = id - u * a.mtiles;
+    int mt, u;
+    place_block(id, total, a.order, a.mtiles, a.by_mtiles, mt, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
     const int bz = a.by_splits(us), split = us - bz * a.splits;
 
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, false)))
 {
     __shared__ __attribute__((aligned(1024))) char lds[attend_fwd_lds(sizeof(T), DT, WM, 2)];
     __shared__ __attribute__((aligned(16))) float bias[2 * attend_fwd_bn(sizeof(T), DT, WM)];
-    attend_fwd_block<T, DT, WM, 2>(a, lds, bias, xcd_order(blockIdx.x, gridDim.x));
+    attend_fwd_block<T, DT, WM, 2>(a, lds, bias, blockIdx.x, gridDim.x);
 }
 
 // Both parts of a shared call in one launch.  The own part has few rows per workgroup whatever the first has.
@@ -277,9 +278,9 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, true))) 
     __shared__ __attribute__((aligned(16))) float bias[NA > NB ? NA : NB];
     const unsigned n = a.first.mtiles * a.first.splits * a.first.rows.Hk;  // (one grid entry)
     if (blockIdx.x < n)
-        attend_fwd_block<T, DT, WM, 2>(a.first, lds, bias, xcd_order(blockIdx.x, n));
+        attend_fwd_block<T, DT, WM, 2>(a.first, lds, bias, blockIdx.x, n);
     else
-        attend_fwd_block<T, DT, OWN, 1>(a.second, lds, bias, xcd_order(blockIdx.x - n, gridDim.x - n));
+        attend_fwd_block<T, DT, OWN, 1>(a.second, lds, bias, blockIdx.x - n, gridDim.x - n);
 }
 
 // One wave per row: the pieces' maxima and sums (a lane each, 64 at a time), then the pieces' sums weighted by them, the two halves

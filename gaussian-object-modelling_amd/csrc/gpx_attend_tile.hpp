@@ -243,12 +243,21 @@ __device__ __forceinline__ int clamped(const int *len, int b, int n)
     return l < 0 ? 0 : (l > n ? n : l);
 }
 
-// Consecutive workgroups go round the 8 XCDs: give each XCD a contiguous piece of the work, so that workgroups that read
-// the same keys share an L2.
-__device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned total)
+// Consecutive workgroups go round the 8 XCDs, and each XCD has an L2 of its own.  Workgroup -> (tile, group), the tiles of a group
+// reading the same keys (or rows): ATTEND_WHOLE_GROUPS gives XCD x the groups x, x + 8, .. with all their tiles, ATTEND_PIECES a
+// contiguous piece of the list of all tiles, ATTEND_SPREAD every eighth tile.
+__device__ __forceinline__ void place_block(unsigned id, unsigned total, int order, int tiles, const DivBy &by_tiles, int &tile, int &group)
 {
-    const unsigned per = total >> 3, rest = total & 7, x = id & 7, at = id >> 3;
-    return x * per + (x < rest ? x : rest) + at;
+    unsigned at = id;
+    if (order != ATTEND_SPREAD)
+        at = id >> 3;
+    if (order == ATTEND_PIECES) {
+        const unsigned per = total >> 3, rest = total & 7, x = id & 7;
+        at += x * per + (x < rest ? x : rest);
+    }
+    const int u = by_tiles(at);
+    tile = at - u * tiles;
+    group = order == ATTEND_WHOLE_GROUPS ? u * 8 + (int)(id & 7) : u;
 }
 
 // ---- memory -> LDS without registers -------------------------------------------------------------------------------------------
