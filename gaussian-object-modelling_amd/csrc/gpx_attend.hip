@@ -106,13 +106,13 @@ int check_data(const gpx_attend_args &a, int which)
     return GPX_OK;
 }
 
-// `pieces` of [0, n) in whole steps of `step`, of at least `least` steps each: where `blocks` workgroups would leave CUs without
-// one, enough pieces that every CU has the `per_cu` it holds
+// `pieces` of [0, n) in whole steps of `step`, of at least `least` steps each: where `blocks` workgroups are less than half
+// of what the CUs hold (`per_cu` each), enough pieces to fill them
 void cut(int64_t blocks, int64_t n, int step, int least, int cus, int per_cu, int *pieces, int *chunk)
 {
     int64_t p = 1;
     const int64_t steps = std::max<int64_t>(1, (n + step - 1) / step);
-    if (blocks < cus && blocks > 0)
+    if (2 * blocks < (int64_t)cus * per_cu && blocks > 0)
         p = std::min<int64_t>((int64_t)cus * per_cu / blocks, steps / least);
     p = std::max<int64_t>(p, 1);
     const int64_t per = (steps + p - 1) / p;

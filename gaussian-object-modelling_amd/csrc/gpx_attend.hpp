@@ -128,20 +128,20 @@ constexpr int attend_lds_per_cu(int bytes) { return bytes <= 38 * 1024 ? 4 : byt
 // workgroups a CU holds: LDS, and the registers of a wave (512 a SIMD lane, so waves per SIMD = workgroups per CU)
 constexpr int attend_fwd_per_cu(int esz, int dt, int wm, bool pair)
 {
-    const int regs = esz == 4 ? (dt == 1 ? 3 : dt <= 2 + !pair ? 2 : 1) : dt <= 2 ? 3 : 2;
+    const int regs = esz == 4 ? (dt == 1 ? 3 : dt <= 3 ? 2 : 1) : dt <= 2 ? 3 : 2;
     const int lds = attend_lds_per_cu(attend_fwd_lds(esz, dt, wm, 2));
     return lds < regs ? lds : regs;
 }
 constexpr int attend_dq_bn(int wm) { return 32 * (4 / wm); }
 constexpr int attend_dq_per_cu(int esz, int dt, int wm)
 {
-    const int regs = esz == 4 && dt > 2 ? 1 : 2;
+    const int regs = esz == 4 ? (dt > 2 ? 1 : 2) : dt <= 2 ? 3 : 2;
     const int lds = attend_lds_per_cu(4 * attend_dq_bn(wm) * attend_row_bytes(esz, dt));
     return lds < regs ? lds : regs;
 }
 constexpr int ATTEND_DKV_KEYS = 128;  // keys of one workgroup of the dK, dV kernel
 constexpr int attend_dkv_br(int esz) { return esz == 2 ? 64 : 32; }
-constexpr int attend_dkv_per_cu(int esz, int dt) { return esz == 2 || dt <= 2 ? 2 : 1; }
+constexpr int attend_dkv_per_cu(int esz, int dt) { return esz == 2 ? (dt <= 2 ? 3 : 2) : dt <= 2 ? 2 : 1; }
 
 template <typename T> void attend_launch_fwd(const AttendFwd &a, hipStream_t st);
 template <typename T> void attend_launch_pair(const AttendPair &a, hipStream_t st);

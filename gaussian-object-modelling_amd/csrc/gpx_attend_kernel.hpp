@@ -42,12 +42,18 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
     const unsigned char *mask = a.keys.mask ? a.keys.mask + bz * a.keys.mask_b : nullptr;
     const unsigned lds0 = lds_offset(lds);
 
-    unsigned ko[FL::N], vo[FL::N];  // the lane's places in a tile, as offsets from its first row
+    // the lane's places in a tile, as offsets from its first row: kept, or formed at every tile where registers are short
+    constexpr bool KEEP = sizeof(T) == 2 || DT <= 2;
+    unsigned ko[KEEP ? FL::N : 1], vo[KEEP ? FL::N : 1];
+    const auto place = [&](int x, int ln, unsigned &k, unsigned &v) {
+        const unsigned c = FL::chunk(x, wave, ln, rw.D), r = FL::row(x, wave, ln);
+        k = c == DMA_OUT ? DMA_OUT : r * ksb + c;
+        v = c == DMA_OUT ? DMA_OUT : r * vsb + c;
+    };
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int x = 0; x < FL::N; ++x) {
-        const unsigned c = FL::chunk(x, wave, lane, rw.D), r = FL::row(x, wave, lane);
-        ko[x] = c == DMA_OUT ? DMA_OUT : r * ksb + c;
-        vo[x] = c == DMA_OUT ? DMA_OUT : r * vsb + c;
+        for (int x = 0; x < FL::N; ++x)
+            place(x, lane, ko[x], vo[x]);
     }
     // mask bytes of the next tile to fetch: for the rows the lane fetches, and for the key it writes the bias of
     unsigned mb[FL::N + 1];
@@ -67,21 +73,24 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
         const u32x4 kd = dma_buffer(kp + (long)n0 * ksb, (unsigned)min((unsigned long long)left * ksb, (unsigned long long)DMA_MOST));
         const u32x4 vd = dma_buffer(vp + (long)n0 * vsb, (unsigned)min((unsigned long long)left * vsb, (unsigned long long)DMA_MOST));
         const unsigned at0 = lds0 + stage * 2 * TILE_B;
-        if (mask) {
+        int ln = lane;
+        if constexpr (!KEEP)
+            asm volatile("" : "+v"(ln));
 #pragma unroll
-            for (int x = 0; x < FL::N; ++x)
-                if (FL::on(x, wave)) {
-                    dma16(kd, mb[x] ? ko[x] : DMA_OUT, at0 + FL::lds(x, wave));
-                    dma16(vd, mb[x] ? vo[x] : DMA_OUT, at0 + TILE_B + FL::lds(x, wave));
+        for (int x = 0; x < FL::N; ++x)
+            if (FL::on(x, wave)) {
+                unsigned k, v;
+                if constexpr (KEEP)
+                    k = ko[x], v = vo[x];
+                else
+                    place(x, ln, k, v);
+                if (mask) {
+                    k = mb[x] ? k : DMA_OUT;
+                    v = mb[x] ? v : DMA_OUT;
                 }
-        } else {
-#pragma unroll
-            for (int x = 0; x < FL::N; ++x)
-                if (FL::on(x, wave)) {
-                    dma16(kd, ko[x], at0 + FL::lds(x, wave));
-                    dma16(vd, vo[x], at0 + TILE_B + FL::lds(x, wave));
-                }
-        }
+                dma16(kd, k, at0 + FL::lds(x, wave));
+                dma16(vd, v, at0 + TILE_B + FL::lds(x, wave));
+            }
         if ((mask || a.tail || n0 + BN > end) && tid < BN)
             bias[stage * BN + tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
     };
