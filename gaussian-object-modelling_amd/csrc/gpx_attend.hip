@@ -249,6 +249,9 @@ AttendKeys keys_of(const gpx_view &k, const gpx_view &v, int64_t n, const int32_
     return s;
 }
 
+// longest key ranges first: ragged batches of up to 64 with more workgroups than run at once
+int sorts(const gpx_attend_args &a, int64_t blocks, int64_t at_once) { return a.k_len && a.batch > 1 && a.batch <= 64 && blocks > at_once; }
+
 template <typename F>
 int by_type(const gpx_attend_args &a, F &&f)
 {
@@ -309,6 +312,7 @@ extern "C" int gpx_attend(const gpx_attend_args *args)
     set_grid(f, p.wm, p.mtiles, p.splits, p.chunk);
     f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
     f.lse = a.lse;
+    f.keys.sort = sorts(a, f.blocks(), cu_count(a) * attend_fwd_per_cu(elem_size(a), attend_dt((int)a.dim), p.wm, false));
     f.slot_rows = (long)(a.batch * a.nq * a.heads);
     if (p.splits > 1) {
         f.pml = (float2 *)((char *)a.workspace + p.ml);
@@ -390,6 +394,7 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.dq = a.dq.p, b.dqb = a.dq.batch, b.dqr = a.dq.row, b.dqh = a.dq.head;
     b.dk = a.dk.p, b.dkb = a.dk.batch, b.dkr = a.dk.row, b.dkh = a.dk.head;
     b.dv = a.dv.p, b.dvb = a.dv.batch, b.dvr = a.dv.row, b.dvh = a.dv.head;
+    b.keys.sort = sorts(a, (int64_t)p.mtiles * p.splits * a.heads_kv * a.batch, cu_count(a) * attend_dq_per_cu(elem_size(a), attend_dt((int)a.dim), p.wm));
     b.q_splits = p.splits, b.q_chunk = p.chunk;
     b.k_splits = p.k_splits, b.k_chunk = p.k_chunk;
     if (p.splits > 1)

@@ -30,6 +30,7 @@ struct AttendKeys {
     const int *len = nullptr;         // rows that count per batch entry (clamped to [0, n]); null: n
     const unsigned char *mask = nullptr;  // nonzero: the row counts; [batch][mask_b]; null: all
     long mask_b = 0;
+    int sort = 0;                     // 1: the batch entries in the order of their lengths, longest first (at most 64 of them)
 };
 
 // Queries are enumerated per (grid batch entry, key head) as packed rows r = n G + g, g the head inside the group of G heads

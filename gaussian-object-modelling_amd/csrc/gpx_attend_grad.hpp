@@ -30,7 +30,8 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
     int mt, u;
     place_block(blockIdx.x, gridDim.x, a.q_order, a.mtiles, a.by_mtiles, mt, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
-    const int bz = a.by_q_splits(us), split = us - bz * a.q_splits;
+    const int turn = a.by_q_splits(us), split = us - turn * a.q_splits;
+    const int bz = nth_longest(a.keys, rw.grid_b, turn);
 
     const RowAt at = row_at(rw, bz, hk, mt * 32 * WM + wm * 32 + (lane & 31));
     const int len = clamped(a.keys.len, bz, a.keys.n);
@@ -229,7 +230,8 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
     int ktile, u;
     place_block(blockIdx.x, gridDim.x, a.k_order, a.ktiles, a.by_ktiles, ktile, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
-    const int bz = a.by_k_splits(us), split = us - bz * a.k_splits;
+    const int turn = a.by_k_splits(us), split = us - turn * a.k_splits;
+    const int bz = nth_longest(a.keys, rw.grid_b, turn);
 
     const int len = clamped(a.keys.len, bz, a.keys.n);
     const auto counts_of = [&](int key) { return key < len && (!a.keys.mask || a.keys.mask[bz * a.keys.mask_b + key]); };

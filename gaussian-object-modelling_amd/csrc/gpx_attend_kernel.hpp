@@ -29,7 +29,8 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
     int mt, u;
     place_block(id, total, a.order, a.mtiles, a.by_mtiles, mt, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
-    const int bz = a.by_splits(us), split = us - bz * a.splits;
+    const int turn = a.by_splits(us), split = us - turn * a.splits;
+    const int bz = nth_longest(a.keys, rw.grid_b, turn);
 
     const RowAt at = row_at(rw, bz, hk, mt * 32 * WM + wm * 32 + (lane & 31));
     const int len = clamped(a.keys.len, bz, a.keys.n);
