@@ -29,7 +29,7 @@ struct DeviceScope {  // the call runs on args->device; the caller's current dev
     }
 };
 
-constexpr int64_t MOST_ROWS = (int64_t)1 << 30;  // row counts, and rows x heads of a call, stay in 32 bits
+constexpr int64_t MOST_ROWS = (int64_t)1 << 28;  // row counts, and rows x heads of a call: byte offsets of their floats stay in 31 bits
 
 int elem_size(const gpx_attend_args &a) { return a.scalar == GPX_F32 ? 4 : 2; }
 
@@ -83,13 +83,23 @@ int check_data(const gpx_attend_args &a, int which)
     const bool rows = a.batch > 0 && a.nq > 0, keys = a.batch > 0 && a.nk > 0, own = a.batch > 0 && a.n_own > 0;
     int rc;
     const int64_t G = a.heads / a.heads_kv;
+    // an output's rows and heads are written by different workgroups
+#define OUTPUT(V_, ON_, N_, H_)                                                                           \
+    if ((rc = check_view(a, a.V_, ON_, N_, 1, #V_)) != GPX_OK)                                            \
+        return rc;                                                                                        \
+    if ((ON_) && (H_) > 1 && a.V_.head < a.dim)                                                           \
+    return fail(GPX_E_BAD_ARG, #V_ ": the heads of an output must not overlap")
 #define VIEW(V_, ON_, N_, G_)                                 \
     if ((rc = check_view(a, a.V_, ON_, N_, G_, #V_)) != GPX_OK) \
     return rc
     VIEW(q, rows, a.nq, G);
     VIEW(k, keys, a.nk, 1);
     VIEW(v, keys, a.nk, 1);
-    VIEW(o, rows, a.nq, 1);
+    if (which == GPX_ATTEND_BACKWARD) {
+        VIEW(o, rows, a.nq, 1);
+    } else {
+        OUTPUT(o, rows, a.nq, a.heads);
+    }
     if (rows && !a.lse)
         return fail(GPX_E_NULL, "Empty data pointer: lse");
     if (which == GPX_ATTEND_SHARED) {
@@ -98,11 +108,16 @@ int check_data(const gpx_attend_args &a, int which)
     }
     if (which == GPX_ATTEND_BACKWARD) {
         VIEW(d_o, rows, a.nq, G);
-        VIEW(dq, rows, a.nq, 1);
-        VIEW(dk, keys, a.nk, 1);
-        VIEW(dv, keys, a.nk, 1);
+        OUTPUT(dq, rows, a.nq, a.heads);
+        OUTPUT(dk, keys, a.nk, a.heads_kv);
+        OUTPUT(dv, keys, a.nk, a.heads_kv);
     }
 #undef VIEW
+#undef OUTPUT
+    if (a.key_mask && a.key_mask_batch < 0)
+        return fail(GPX_E_BAD_ARG, "key_mask_batch must not be negative");
+    if (which == GPX_ATTEND_SHARED && (a.q_len || a.k_len || a.key_mask))
+        return fail(GPX_E_BAD_ARG, "gpx_attend_shared takes own_len only");
     return GPX_OK;
 }
 
@@ -335,8 +350,6 @@ extern "C" int gpx_attend_shared(const gpx_attend_args *args)
     if (rc != GPX_OK)
         return rc;
     const gpx_attend_args &a = *args;
-    if (a.q_len || a.k_len || a.key_mask)
-        return fail(GPX_E_BAD_ARG, "gpx_attend_shared takes own_len only");
     if (a.batch == 0 || a.nq == 0)
         return GPX_OK;
     AttendFwd f;

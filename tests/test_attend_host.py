@@ -27,6 +27,8 @@ def args(at, **kv):
     for p in ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv", "k_own", "v_own"):
         d[p] = 4096
     for p in NAMES:
+        if p in ("qh", "kh", "vh", "oh", "gh", "dqh", "dkh", "dvh", "koh", "voh"):
+            d[p] = 64
         if p in ("qr", "kr", "vr", "orow", "gr", "dqr", "dkr", "dvr", "kor", "vor"):
             d[p] = 256
     d.update(kv)
@@ -38,7 +40,7 @@ BAD = [(dict(scalar=3), -10), (dict(scalar=-1), -10), (dict(heads=3), -10), (dic
        (dict(scale=0.0), -10), (dict(scale=-1.0), -10), (dict(scale=math.nan), -10), (dict(scale=math.inf), -10), (dict(scale=1e300), -10),
        (dict(nq=2 ** 31), -10), (dict(nk=2 ** 31), -10), (dict(batch=2 ** 20, nq=2 ** 20), -10), (dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1),
        (dict(o=0), -1), (dict(lse=0), -1), (dict(q=4098), -10), (dict(kb=3), -10), (dict(vr=4), -10), (dict(qh=-8), -10), (dict(oh=1), -10),
-       (dict(kr=0), -10), (dict(vr=56), -10), (dict(kr=2 ** 22 + 8), -10), (dict(qh=2 ** 27), -10)]
+       (dict(kr=0), -10), (dict(vr=56), -10), (dict(kr=2 ** 22 + 8), -10), (dict(qh=2 ** 27), -10), (dict(nq=2 ** 28 + 1), -10), (dict(batch=2 ** 14, nq=2 ** 13, heads=4), -10)]
 
 
 @pytest.mark.parametrize("kv,code", BAD, ids=lambda x: str(x))
@@ -58,6 +60,19 @@ def test_entry_points_refuse_null(gpx, at):
     assert at._entry(at.BACKWARD)(args(at, dk=0)) == gpx.E_NULL
     assert at._entry(at.BACKWARD)(args(at, d_o=0)) == gpx.E_NULL
     assert at._entry(at.SHARED)(args(at, n_own=4, k_own=0)) == gpx.E_NULL
+
+
+def test_outputs_do_not_overlap(gpx, at):
+    assert at._entry(at.FORWARD)(args(at, oh=0)) == gpx.E_BAD_ARG
+    assert at._entry(at.SHARED)(args(at, oh=56)) == gpx.E_BAD_ARG
+    for h in ("dqh", "dkh", "dvh"):
+        assert at._entry(at.BACKWARD)(args(at, **{h: 56})) == gpx.E_BAD_ARG
+
+
+def test_masks_that_a_call_does_not_take(gpx, at):
+    for kv in (dict(q_len=4096), dict(k_len=4096), dict(key_mask=4096)):
+        assert at._entry(at.SHARED)(args(at, **kv)) == gpx.E_BAD_ARG
+    assert at._entry(at.FORWARD)(args(at, key_mask=4096, key_mask_batch=-1)) == gpx.E_BAD_ARG
 
 
 def test_workspace_sizes(gpx, at):

@@ -120,6 +120,36 @@ def test_rows_split_over_workgroups_in_the_gradient_of_few_keys(at, t):
             hold(name, got[name], *want[name])
 
 
+# enough (batch, head) pairs to fill the card: workgroups of 64 and of 128 rows, in several orders over the XCDs
+WIDE = [(16, 40, 97, 16, 16, 32), (16, 70, 97, 16, 16, 64), (16, 40, 97, 16, 16, 72), (17, 70, 65, 16, 16, 96), (16, 40, 130, 16, 16, 128),
+        (19, 70, 130, 14, 14, 120), (2, 100, 150, 8, 4, 64)]
+
+
+@pytest.mark.parametrize("kind", ["none", "len+mask+rows"])
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", WIDE, ids=lambda s: "x".join(map(str, s)))
+def test_many_heads(at, t, shape, kind):
+    want, got = both(at, t, shape, kind, 7)
+    for name in got:
+        hold(name, got[name], *want[name])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_ragged_batch_of_many_workgroups(at, t):
+    """More workgroups than run at once: the batch entries are taken in the order of their lengths (ties, zeros and all)."""
+    b, nq, nk, hq, hk, d = 24, 1100, 150, 4, 4, 32
+    q, k, v, do = inputs(t, b, nq, nk, hq, hk, d, 13)
+    n = torch.randint(0, nk + 1, (b,), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+    n[3] = n[4] = n[11] = 77
+    n[0] = n[23] = 0
+    want = ora.attend(q, k, v, d ** -0.5, ora.seen_of(b, nq, nk, n), do)
+    g = [x.cuda() for x in (q, k, v, do)]
+    o, lse = at.attend(*g[:3], k_len=n.cuda())
+    got = dict(zip(("dq", "dk", "dv"), at.attend_backward(g[3], *g[:3], o, lse, k_len=n.cuda())), o=o, lse=lse)
+    for name in got:
+        hold(name, got[name], *want[name])
+
+
 def test_no_entries_and_no_queries(at):
     q = torch.randn(2, 3, 4, 64, device="cuda")
     e = torch.empty(2, 0, 2, 64, device="cuda")
@@ -226,7 +256,8 @@ def test_context_beyond_32_bit_offsets(at):
 
 
 SHARED = [(2, 1, 277, 15, 8, 8, 64), (5, 1, 1000, 40, 8, 2, 128), (3, 4, 600, 9, 6, 2, 80), (17, 5, 2000, 64, 3, 1, 32), (1, 1, 1, 1, 1, 1, 8),
-          (40, 1, 300, 130, 4, 4, 96), (2, 7, 0, 20, 2, 1, 64), (2, 3, 50, 0, 2, 2, 64)]
+          (40, 1, 300, 130, 4, 4, 96), (2, 7, 0, 20, 2, 1, 64), (2, 3, 50, 0, 2, 2, 64), (40, 1, 2000, 30, 16, 16, 64), (70, 1, 2100, 30, 16, 16, 128),
+          (35, 2, 2100, 30, 16, 16, 80), (70, 1, 2100, 257, 16, 16, 32)]
 
 
 @pytest.mark.parametrize("t", list(TYPES))
