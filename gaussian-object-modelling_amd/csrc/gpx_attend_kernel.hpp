@@ -9,11 +9,19 @@ namespace gpx {
 namespace attend {
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
+// o_i = sum_j 2^(c s_ij - m_i) v_j / sum_j 2^(c s_ij - m_i), s = Q K^T, c = scale log2(e), in one pass over the keys with a running
+// maximum m and sum l per row.
 // One workgroup of 4 waves: WM waves along the rows (32 packed rows each), WK = 4 / WM along the keys.  Scores are formed
 // TRANSPOSED, S^T = K Q^T: a lane then holds one row's weights (its column), the running maximum and sum of a row are one
 // register per lane, and S^T turns into the operand of O^T = V^T P^T without leaving the lane (gpx_attend_tile.hpp).
 // Keys and values are read from memory once per 32 WM rows, as tiles of BN rows, two of them in LDS: while one is worked on the
-// next is on its way.
+// next is on its way.  64 keys a wave and step for the 16-bit types with WM = 4 (32: as fast at 64 and slower at 96 features).
+// What bounds it (bf16; the library's 8192^3 product reaches 1067 TFLOP/s on the same card):
+//   16384 x 16384, 16 heads of 128   2.06 ms, 1066 TFLOP/s: the matrix cores at the card's power limit (clock 1.9-2.1 GHz; without
+//                                    the softmax 2.01, without any fetch 1.95)
+//   32768 x 724, 8 heads of 64       67 us, 727 TFLOP/s: vector issue (153 instructions a tile and wave, 128 of them the softmax's,
+//                                    beside 16 matrix instructions) and three rounds of 12-tile workgroups
+//   4 x 65536, 32/8 heads of 128 x 3 156 us, 5.2 TB/s: memory
 // STAGES == 1 has one tile at a time (the own part of a shared call: short ranges, many workgroups a CU).
 template <typename T, int DT, int WM, int STAGES>
 __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, float *bias, unsigned id, unsigned total)
@@ -275,7 +283,8 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, false)))
     attend_fwd_block<T, DT, WM, 2>(a, lds, bias, blockIdx.x, gridDim.x);
 }
 
-// Both parts of a shared call in one launch.  The own part has few rows per workgroup whatever the first has.
+// Both parts of a shared call in one launch (two launches: 64 members over 131072 entries 242 us, one: 220).  The own part has few
+// rows per workgroup whatever the first has.  That case now: 204 us = 3.5 TB/s and 675 TFLOP/s at once, 0.75 of either's rate.
 template <typename T, int DT>
 constexpr int own_wm() { return attend_least_wm(sizeof(T), DT); }
 template <typename T, int DT, int WM>
@@ -294,7 +303,8 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, true))) 
 }
 
 // One wave per row: the pieces' maxima and sums (a lane each, 64 at a time), then the pieces' sums weighted by them, the two halves
-// of the wave taking every other piece, four values a lane.
+// of the wave taking every other piece, four values a lane and four pieces in flight (384 rows x 21 pieces of 128: 4.4 us; one
+// piece at a time: 14 us).
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendJoin a)
 {
