@@ -158,6 +158,11 @@ def lib():
     L.gpx_debug_reload.restype = None
     L.gpx_model_replicate.restype = C.c_int
     L.gpx_model_replicate.argtypes = [vp, C.c_int, C.POINTER(C.c_int), C.POINTER(vp)]
+    for f in (L.gpx_attend, L.gpx_attend_backward, L.gpx_attend_shared):  # gpx_attend_args as bytes; attend.py goes through gpx_torch.so
+        f.restype = C.c_int
+        f.argtypes = [C.c_char_p]
+    L.gpx_attend_workspace.restype = C.c_int
+    L.gpx_attend_workspace.argtypes = [C.c_char_p, C.c_int, C.POINTER(C.c_size_t)]
     L.gpx_dev_kbuild.restype = C.c_int
     L.gpx_dev_kbuild.argtypes = [C.POINTER(Kernel), C.c_int, C.c_size_t, C.c_size_t, vp, vp, vp, vp, vp, vp, vp]
     L.gpx_dev_kqp.restype = C.c_int

@@ -2,6 +2,7 @@
 import ctypes as C
 import importlib
 import math
+import struct
 
 import pytest
 
@@ -10,8 +11,25 @@ import attend_oracle as ora
 torch = pytest.importorskip("torch")
 
 
+class Abi:
+    """The C entry points, called with the bytes of a gpx_attend_args."""
+    FORWARD, BACKWARD, SHARED = range(3)
+    _ARGS = struct.Struct("@iiqqqqqqqd" + "Pqqq" * 4 + "PPPPq" + "Pqqq" * 6 + "PPQP")
+
+    def __init__(self, L):
+        self.calls = (L.gpx_attend, L.gpx_attend_backward, L.gpx_attend_shared, L.gpx_attend_workspace)
+
+    def _entry(self, i):
+        return self.calls[i]
+
+
 @pytest.fixture(scope="module")
 def at(gpx):
+    return Abi(gpx.lib())
+
+
+@pytest.fixture(scope="module")
+def front(gpx):
     return importlib.import_module("gaussian-object-modelling_amd.attend")
 
 
@@ -94,15 +112,18 @@ def test_no_gpu_no_result(gpx, at):
     assert at._entry(at.FORWARD)(args(at)) == gpx.E_NO_DEVICE
 
 
-def test_torch_front_refuses(gpx, at):
+def test_torch_front_refuses(gpx, front):
     z = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t)  # noqa: E731
     q, k = z(2, 3, 4, 64), z(2, 5, 2, 64)
-    for call in (lambda: at.attend(q, k, k),                                    # no CPU path
-                 lambda: at.attend(q[0], k, k), lambda: at.attend(q, k[0], k), lambda: at.attend(q.double(), k.double(), k.double()),
-                 lambda: at.attend(q, z(2, 5, 3, 64), z(2, 5, 3, 64)), lambda: at.attend_shared(q, k, k, k, k),
-                 lambda: at.attend(None, k, k)):
-        with pytest.raises(gpx.GpxError):
+    for call in (lambda: front.attend(q, k, k),                                    # no CPU path
+                 lambda: front.attend(q[0], k, k), lambda: front.attend(q, k[0], k), lambda: front.attend(q.double(), k.double(), k.double()),
+                 lambda: front.attend(q, z(2, 5, 3, 64), z(2, 5, 3, 64)), lambda: front.attend_shared(q, k, k, k, k),
+                 lambda: front.attend_backward(q, q, k, k, q, z(2, 4, 3))):
+        with pytest.raises(gpx.GpxError) as e:
             call()
+        assert e.value.code == gpx.E_BAD_ARG and e.value.message
+    with pytest.raises(TypeError):
+        front.attend(q, k, None)
 
 
 @pytest.mark.parametrize("t,n", [(torch.float32, 300), (torch.float16, 300), (torch.bfloat16, 12)], ids=str)

@@ -150,6 +150,37 @@ def test_ragged_batch_of_many_workgroups(at, t):
         hold(name, got[name], *want[name])
 
 
+def test_refusals(gpu, at):
+    q, k, v, do = (x.cuda() for x in inputs("f32", 2, 3, 5, 4, 2, 64, 0))
+    o, lse = at.attend(q, k, v)
+    n = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    bad = [lambda: at.attend(q, k.half(), v), lambda: at.attend(q, k.cpu(), v), lambda: at.attend(q, k, v[:, :4]), lambda: at.attend(q, k, v[..., :32]),
+           lambda: at.attend(q[..., :60], k[..., :60], v[..., :60]), lambda: at.attend(q, k, v, scale=0.0), lambda: at.attend(q, k, v, scale=math.inf),
+           lambda: at.attend(q, k, v, k_len=n.long()), lambda: at.attend(q, k, v, k_len=n[:1]), lambda: at.attend(q, k, v, k_len=n.cpu()),
+           lambda: at.attend(q, k, v, q_len=n[None]), lambda: at.attend(q, k, v, key_mask=torch.ones(2, 4, dtype=torch.bool, device="cuda")),
+           lambda: at.attend(q, k, v, key_mask=torch.ones(2, 5, device="cuda")),
+           lambda: at.attend(q, k, v, key_mask=torch.ones(2, 10, dtype=torch.bool, device="cuda")[:, ::2]),
+           lambda: at.attend(q[:, :, :3], k, v), lambda: at.attend(q, k[:, :, :0], v[:, :, :0]), lambda: at.attend(q.double(), k.double(), v.double()),
+           lambda: at.attend_backward(do, q, k, v, o, lse.half()), lambda: at.attend_backward(do, q, k, v, o, lse[:, :2]),
+           lambda: at.attend_backward(do[:1], q, k, v, o, lse), lambda: at.attend_backward(do, q, k, v, o.half(), lse),
+           lambda: at.attend_shared(q, k, v, k, v), lambda: at.attend_shared(q, k[0], v[0], k[:, :, :1], v), lambda: at.attend_shared(q, k[0], v[0, :4], k, v),
+           lambda: at.attend_shared(q, k[0], v[0], k, v, n[:1])]
+    for i, call in enumerate(bad):
+        with pytest.raises(gpu.GpxError) as e:
+            call()
+        assert e.value.code in (gpu.E_BAD_ARG, gpu.E_SIZE_MISMATCH), i
+    o2, lse2 = at.attend(q, k, v)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+def test_inputs_that_require_gradients(at):
+    """Nothing is recorded, views and copies included."""
+    q, k, v, _ = (x.cuda().requires_grad_() for x in inputs("f32", 2, 3, 5, 4, 2, 64, 0))
+    o, lse = at.attend(q, k.permute(0, 1, 3, 2).contiguous().permute(0, 1, 3, 2), v)
+    o2, _ = at.attend_shared(q, k[0], v[0], k, v)
+    assert not o.requires_grad and not lse.requires_grad and not o2.requires_grad
+
+
 def test_no_entries_and_no_queries(at):
     q = torch.randn(2, 3, 4, 64, device="cuda")
     e = torch.empty(2, 0, 2, 64, device="cuda")
