@@ -12,7 +12,6 @@ recorded by autograd.
 """
 import importlib.machinery
 import importlib.util
-import math
 import os
 
 import torch
@@ -47,16 +46,16 @@ def attend(q, k, v, scale=None, k_len=None, key_mask=None, q_len=None):
     """o [batch, nq, heads, dim] and lse [batch, heads, nq] (float32) of queries q [batch, nq, heads, dim] over k, v
     [batch, nk, heads_kv, dim].  scale: dim ** -0.5 unless given.  k_len, q_len: int32 [batch], entries and queries that count
     (the others' o is zero, lse -inf); key_mask: bool [batch, nk], True where the entry counts."""
-    return (_loaded or ext()).attend(q, k, v, math.nan if scale is None else scale, k_len, key_mask, q_len, _stream(q))
+    return (_loaded or ext()).attend(q, k, v, scale, k_len, key_mask, q_len, _stream(q))
 
 
 def attend_backward(d_o, q, k, v, o, lse, scale=None, k_len=None, key_mask=None, q_len=None):
     """dq, dk, dv for the gradient d_o of attend's o; o and lse as attend returned them, the other arguments as it got them."""
-    return (_loaded or ext()).attend_backward(d_o, q, k, v, o, lse, math.nan if scale is None else scale, k_len, key_mask, q_len, _stream(q))
+    return (_loaded or ext()).attend_backward(d_o, q, k, v, o, lse, scale, k_len, key_mask, q_len, _stream(q))
 
 
 def attend_shared(q, k, v, k_own, v_own, own_len=None, scale=None):
     """o and lse (as attend) of a batch over ONE context: q [batch, nq, heads, dim]; k, v [nk, heads_kv, dim], which every query
     sees; k_own, v_own [batch, n_own, heads_kv, dim], of which own_len[b] (int32 [batch]; None: all) exist, the rows of the nq
     queries last: query i sees the own entries j < own_len[b] - (nq - 1 - i).  The context is read once for the whole batch."""
-    return (_loaded or ext()).attend_shared(q, k, v, k_own, v_own, own_len, math.nan if scale is None else scale, _stream(q))
+    return (_loaded or ext()).attend_shared(q, k, v, k_own, v_own, own_len, scale, _stream(q))

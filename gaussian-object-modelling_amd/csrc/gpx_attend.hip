@@ -221,6 +221,17 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
     return p;
 }
 
+// a grid holds less than 2^32 threads: 2^24 workgroups
+bool launches_fit(const gpx_attend_args &a, int which, const Plan &p)
+{
+    const int64_t most = ((int64_t)1 << 24) - 1, pairs = a.heads_kv * a.batch, rows = a.batch * a.nq * a.heads;
+    if (which == GPX_ATTEND_SHARED)
+        return (int64_t)p.mtiles * p.splits * a.heads_kv + (int64_t)p.own_mtiles * p.own_splits * pairs <= most && rows / 4 < most;
+    if ((int64_t)p.mtiles * p.splits * pairs > most || (p.splits > 1 && rows / 4 >= most))
+        return false;
+    return which == GPX_ATTEND_FORWARD || (int64_t)p.ktiles * p.k_splits * pairs <= most;
+}
+
 int cu_count(const gpx_attend_args &a)
 {
     int dev = a.device;
@@ -295,6 +306,8 @@ int begin(const gpx_attend_args *pa, int which, DeviceScope &scope, Plan *plan)
     if (rc != GPX_OK)
         return rc;
     *plan = plan_of(*pa, which, cu_count(*pa));
+    if (!launches_fit(*pa, which, *plan))
+        return fail(GPX_E_BAD_ARG, "too many rows for one call");
     if (plan->total > pa->workspace_bytes || (plan->total && (!pa->workspace || (uintptr_t)pa->workspace % 256)))
         return fail(GPX_E_SIZE_MISMATCH, "workspace: gpx_attend_workspace bytes on a 256-byte boundary are needed");
     return GPX_OK;
@@ -309,7 +322,10 @@ extern "C" int gpx_attend_workspace(const gpx_attend_args *args, int which, size
     const int rc = check_args(args, which);
     if (rc != GPX_OK)
         return rc;
-    *bytes = plan_of(*args, which, cu_count(*args)).total;
+    const Plan p = plan_of(*args, which, cu_count(*args));
+    if (!launches_fit(*args, which, p))
+        return fail(GPX_E_BAD_ARG, "too many rows for one call");
+    *bytes = p.total;
     return GPX_OK;
 }
 

@@ -232,8 +232,12 @@ __device__ __forceinline__ void load_row_frags(Frag<T> (&f)[2 * DT], const T *p,
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             z[j] = (T)0.0f;
-        if (valid && d < D)
-            z = *reinterpret_cast<const x8<T> *>(p + d);
+        if (valid && d < D) {
+            if constexpr (sizeof(T) == 4)  // (16-byte boundaries, not 32)
+                z = __builtin_shufflevector(*reinterpret_cast<const f32x4 *>(p + d), *reinterpret_cast<const f32x4 *>(p + d + 4), 0, 1, 2, 3, 4, 5, 6, 7);
+            else
+                z = *reinterpret_cast<const x8<T> *>(p + d);
+        }
         f[t] = Frag<T>::of(z);
     }
 }

@@ -45,7 +45,7 @@ struct Call {
     int copies = 0;
 
     // the checks of q; hk: the key heads
-    Call(const Tensor &q_, int64_t hk, double scale) : q(q_)
+    Call(const Tensor &q_, int64_t hk, std::optional<double> scale) : q(q_)
     {
         if (q.dim() != 4)
             refuse("q must be a [batch, row, head, dim] tensor");
@@ -64,7 +64,7 @@ struct Call {
         if (a.dim < 8 || a.dim > 128 || a.dim % 8)
             refuse("dim must be a multiple of 8 up to 128");
         group = a.heads / hk;
-        a.scale = std::isnan(scale) ? 1.0 / std::sqrt((double)a.dim) : scale;
+        a.scale = scale ? *scale : 1.0 / std::sqrt((double)a.dim);
         like = q.options();
     }
 
@@ -135,7 +135,7 @@ int64_t heads_of(const Tensor &k, int64_t dims)
     return k.size(dims - 2);
 }
 
-std::tuple<Tensor, Tensor> attend(const Tensor &q, const Tensor &k, const Tensor &v, double scale, const OptTensor &k_len,
+std::tuple<Tensor, Tensor> attend(const Tensor &q, const Tensor &k, const Tensor &v, std::optional<double> scale, const OptTensor &k_len,
                                   const OptTensor &key_mask, const OptTensor &q_len, uint64_t stream)
 {
     Call c(q, heads_of(k, 4), scale);
@@ -156,7 +156,7 @@ std::tuple<Tensor, Tensor> attend(const Tensor &q, const Tensor &k, const Tensor
 }
 
 std::tuple<Tensor, Tensor, Tensor> attend_backward(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &o,
-                                                   const Tensor &lse, double scale, const OptTensor &k_len, const OptTensor &key_mask,
+                                                   const Tensor &lse, std::optional<double> scale, const OptTensor &k_len, const OptTensor &key_mask,
                                                    const OptTensor &q_len, uint64_t stream)
 {
     Call c(q, heads_of(k, 4), scale);
@@ -183,7 +183,7 @@ std::tuple<Tensor, Tensor, Tensor> attend_backward(const Tensor &d_o, const Tens
 }
 
 std::tuple<Tensor, Tensor> attend_shared(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &k_own, const Tensor &v_own,
-                                         const OptTensor &own_len, double scale, uint64_t stream)
+                                         const OptTensor &own_len, std::optional<double> scale, uint64_t stream)
 {
     const int64_t hk = heads_of(k, 3);
     if (heads_of(v, 3) != hk || heads_of(k_own, 4) != hk)

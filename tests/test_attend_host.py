@@ -93,6 +93,15 @@ def test_masks_that_a_call_does_not_take(gpx, at):
     assert at._entry(at.FORWARD)(args(at, key_mask=4096, key_mask_batch=-1)) == gpx.E_BAD_ARG
 
 
+def test_more_workgroups_than_a_grid_holds(gpx, at):
+    n = C.c_size_t(0)
+    for which in range(3):
+        kv = dict(batch=2 ** 24, nq=1, nk=1, n_own=1, heads=1, heads_kv=1)
+        assert at._entry(3)(args(at, **kv), which, C.byref(n)) == gpx.E_BAD_ARG
+        kv["batch"] = 2 ** 23
+        assert at._entry(3)(args(at, **kv), which, C.byref(n)) == gpx.OK
+
+
 def test_workspace_sizes(gpx, at):
     def need(which, **kv):
         n = C.c_size_t(0)

@@ -155,7 +155,7 @@ def test_refusals(gpu, at):
     o, lse = at.attend(q, k, v)
     n = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
     bad = [lambda: at.attend(q, k.half(), v), lambda: at.attend(q, k.cpu(), v), lambda: at.attend(q, k, v[:, :4]), lambda: at.attend(q, k, v[..., :32]),
-           lambda: at.attend(q[..., :60], k[..., :60], v[..., :60]), lambda: at.attend(q, k, v, scale=0.0), lambda: at.attend(q, k, v, scale=math.inf),
+           lambda: at.attend(q[..., :60], k[..., :60], v[..., :60]), lambda: at.attend(q, k, v, scale=0.0), lambda: at.attend(q, k, v, scale=math.nan), lambda: at.attend(q, k, v, scale=math.inf),
            lambda: at.attend(q, k, v, k_len=n.long()), lambda: at.attend(q, k, v, k_len=n[:1]), lambda: at.attend(q, k, v, k_len=n.cpu()),
            lambda: at.attend(q, k, v, q_len=n[None]), lambda: at.attend(q, k, v, key_mask=torch.ones(2, 4, dtype=torch.bool, device="cuda")),
            lambda: at.attend(q, k, v, key_mask=torch.ones(2, 5, device="cuda")),
@@ -250,6 +250,12 @@ def test_layouts(at, t):
     off = []
     for x in g:
         w = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape)
+        w.copy_(x)
+        off.append(w)
+    same(off)
+    off = []
+    for x in g:  # on a 16-byte boundary, not a 32-byte one
+        w = torch.empty(x.numel() + 16 // x.element_size(), dtype=x.dtype, device="cuda")[16 // x.element_size():].view(x.shape)
         w.copy_(x)
         off.append(w)
     same(off)
