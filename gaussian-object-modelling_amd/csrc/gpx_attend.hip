@@ -96,7 +96,7 @@ int check_data(const gpx_attend_args &a, int which)
     VIEW(k, keys, a.nk, 1);
     VIEW(v, keys, a.nk, 1);
     if (which == GPX_ATTEND_BACKWARD) {
-        VIEW(o, rows, a.nq, 1);
+        VIEW(o, rows, a.nq, G);
     } else {
         OUTPUT(o, rows, a.nq, a.heads);
     }
@@ -155,6 +155,7 @@ struct Plan {
     int splits = 1, chunk = 0;          // forward / the shared context
     int own_splits = 0, own_chunk = 0;  // the own part
     int mtiles = 1, own_mtiles = 1, ktiles = 1;  // workgroups along the rows, along the keys (backward)
+    bool fused = false;
     int k_splits = 1, k_chunk = 0;      // backward, dK dV: pieces of the rows
     size_t ml = 0, po = 0, pk = 0, pv = 0, total = 0;  // offsets into the workspace (ml: the row statistics in a backward call)
 };
@@ -206,7 +207,13 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
     p.ktiles = (int)blocks_of(a.nk, ATTEND_DKV_KEYS);
     cut(blocks, a.nk, attend_dq_bn(wm), least_steps(wm), cus, attend_dq_per_cu(esz, dt, wm), &p.splits, &p.chunk);
     cut(p.ktiles * a.heads_kv * a.batch, R, attend_dkv_br(esz), LEAST_DKV_STEPS, cus, attend_dkv_per_cu(esz, dt), &p.k_splits, &p.k_chunk);
-    size_t at = up(2 * rid * sizeof(float));
+    // One launch for dQ and dK, dV together where all their workgroups run at once, or in two rounds of two and more a CU: two small
+    // objects 29 -> 20 us.  (With 96 and 128 features the joint kernel is alone on its CU: four batches of 1232 x 874 took 118 us
+    // instead of 97.)
+    const int both = attend_both_per_cu(esz, dt, wm);
+    p.fused = R > 0 && a.nk > 0 &&
+              ((int64_t)p.mtiles * p.splits + (int64_t)p.ktiles * p.k_splits) * a.heads_kv * a.batch <= (int64_t)cus * both * (both > 1 ? 2 : 1);
+    size_t at = p.fused ? 0 : up(2 * rid * sizeof(float));
     p.po = at;
     if (p.splits > 1)
         at = up(at + p.splits * rid * a.dim * sizeof(float));
@@ -427,6 +434,7 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
     b.dk = a.dk.p, b.dkb = a.dk.batch, b.dkr = a.dk.row, b.dkh = a.dk.head;
     b.dv = a.dv.p, b.dvb = a.dv.batch, b.dvr = a.dv.row, b.dvh = a.dv.head;
     b.keys.sort = sorts(a, (int64_t)p.mtiles * p.splits * a.heads_kv * a.batch, cu_count(a) * attend_dq_per_cu(elem_size(a), attend_dt((int)a.dim), p.wm));
+    b.fused = p.fused;
     b.q_splits = p.splits, b.q_chunk = p.chunk;
     b.k_splits = p.k_splits, b.k_chunk = p.k_chunk;
     if (p.splits > 1)

@@ -100,6 +100,7 @@ struct AttendBwd {
                              // weights); <dO, O>
     void *dq = nullptr, *dk = nullptr, *dv = nullptr;
     long dqb = 0, dqr = 0, dqh = 0, dkb = 0, dkr = 0, dkh = 0, dvb = 0, dvr = 0, dvh = 0;
+    int fused = 0;                   // dQ and dK, dV in one launch
     int q_splits = 1, q_chunk = 0;   // dQ: pieces of the key range
     int wm = 4;                      // dQ: waves along the rows
     int mtiles = 1, ktiles = 1;      // workgroups along the rows (dQ) and along the keys (dK, dV)
@@ -134,15 +135,24 @@ constexpr int attend_fwd_per_cu(int esz, int dt, int wm, bool pair)
     return lds < regs ? lds : regs;
 }
 constexpr int attend_dq_bn(int wm) { return 32 * (4 / wm); }
+constexpr int attend_dq_lds(int esz, int dt, int wm) { return 4 * attend_dq_bn(wm) * attend_row_bytes(esz, dt); }
 constexpr int attend_dq_per_cu(int esz, int dt, int wm)
 {
     const int regs = esz == 4 ? (dt > 2 ? 1 : 2) : dt <= 2 ? 3 : 2;
-    const int lds = attend_lds_per_cu(4 * attend_dq_bn(wm) * attend_row_bytes(esz, dt));
+    const int lds = attend_lds_per_cu(attend_dq_lds(esz, dt, wm));
     return lds < regs ? lds : regs;
 }
 constexpr int ATTEND_DKV_KEYS = 128;  // keys of one workgroup of the dK, dV kernel
 constexpr int attend_dkv_br(int esz) { return esz == 2 ? 64 : 32; }
 constexpr int attend_dkv_per_cu(int esz, int dt) { return esz == 2 ? (dt <= 2 ? 3 : 2) : dt <= 2 ? 2 : 1; }
+
+constexpr int attend_dkv_lds(int esz, int dt, bool own) { return (own ? 6 : 4) * attend_dkv_br(esz) * attend_row_bytes(esz, dt); }
+constexpr int attend_both_per_cu(int esz, int dt, int wm)
+{
+    const int q = attend_dq_per_cu(esz, dt, wm), k = attend_dkv_per_cu(esz, dt), lds = attend_lds_per_cu(attend_dkv_lds(esz, dt, true));
+    const int regs = q < k ? q : k;
+    return lds < regs ? lds : regs;
+}
 
 template <typename T> void attend_launch_fwd(const AttendFwd &a, hipStream_t st);
 template <typename T> void attend_launch_pair(const AttendPair &a, hipStream_t st);

@@ -18,22 +18,20 @@ namespace gpx {
 namespace attend {
 
 // dQ: waves and tiles as in the forward kernel.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
-// The first piece of the key range also leaves each row's statistics for the dK, dV kernel, which runs behind this one.
+// The first piece of the key range also leaves each row's statistics for the dK, dV kernel, where that runs behind this one.
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void attend_dq_kernel(AttendBwd a)
+__device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, float *bias, unsigned id, unsigned total)
 {
     using TL = Tile<T, DT>;
     constexpr int WK = 4 / WM, KT = 32, BN = attend_dq_bn(WM);
     using FL = Fill<T, DT, BN>;
     constexpr int TILE_B = BN * TL::ROWB;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];
-    __shared__ __attribute__((aligned(16))) float bias[2][BN];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int wm = wave % WM, wk = wave / WM;
     const AttendRows &rw = a.rows;
     int mt, u;
-    place_block(blockIdx.x, gridDim.x, a.q_order, a.mtiles, a.by_mtiles, mt, u);
+    place_block(id, total, a.q_order, a.mtiles, a.by_mtiles, mt, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
     const int turn = a.by_q_splits(us), split = us - turn * a.q_splits;
     const int bz = nth_longest(a.keys, rw.grid_b, turn);
@@ -88,7 +86,7 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
                 }
         }
         if ((mask || n0 + BN > end) && tid < BN)
-            bias[stage][tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
+            bias[stage * BN + tid] = n0 + tid < end && (!mask || mb[FL::N]) ? 0.0f : NEG_INF;
     };
     if (begin < end) {
         look(begin);
@@ -116,7 +114,7 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
             lse = from * 1.44269504088896f;
         else
             dd = 0.0f;
-        if (split == 0 && wk == 0 && half == 0 && at.exists) {
+        if (!a.fused && split == 0 && wk == 0 && half == 0 && at.exists) {
             a.stat[rid] = lse;
             a.stat[(long)rw.grid_b * rw.Hk * rw.G * rw.M + rid] = dd;
         }
@@ -140,7 +138,7 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
         if constexpr (EDGE) {  // -inf where the key does not count: its weight, and with it dS, is zero
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage][wk * KT + 8 * x + 4 * half]);
+                const f32x4 w = *reinterpret_cast<const f32x4 *>(&bias[stage * BN + wk * KT + 8 * x + 4 * half]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     sc[4 * x + j] = w[j];
@@ -214,15 +212,16 @@ __global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void at
 
 // dK, dV: two waves per SIMD at 128 features (254 registers; with one wave and 372 registers 1767 us where it now takes 1010).  4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one
 // key, then dV^T += dO^T P and dK^T += Q^T dS.
-template <typename T, int DT>
-__global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void attend_dkv_kernel(AttendBwd a)
+// OWN: in one launch with dQ; <dO, O> is formed here, from tiles of O beside those of dO, once per tile by all threads.
+template <typename T, int DT, bool OWN>
+__device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, float *stat, unsigned id, unsigned total)
 {
     using TL = Tile<T, DT>;
     constexpr int BR = attend_dkv_br(sizeof(T));
     using FL = Fill<T, DT, BR>;
-    constexpr int TILE_B = BR * TL::ROWB;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];      // [stage][Q, dO]
-    __shared__ __attribute__((aligned(1024))) float stat[2][2][64];      // [stage][lse, <dO, O>][row]
+    constexpr int TILE_B = BR * TL::ROWB, STAGE_B = (OWN ? 3 : 2) * TILE_B;
+    // lds: [stage][Q, dO (, O)]; stat: [stage][lse, <dO, O>][64] (OWN: lse as it is in memory), OWN: then lse in log2 units and <dO, O>
+    float *own = stat + 4 * 64;
 
     // 128 features fill the registers: what follows from the lane's number is formed again where it is needed, not kept
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
     };
     const AttendRows &rw = a.rows;
     int ktile, u;
-    place_block(blockIdx.x, gridDim.x, a.k_order, a.ktiles, a.by_ktiles, ktile, u);
+    place_block(id, total, a.k_order, a.ktiles, a.by_ktiles, ktile, u);
     const int us = rw.by_hk(u), hk = u - us * rw.Hk;
     const int turn = a.by_k_splits(us), split = us - turn * a.k_splits;
     const int bz = nth_longest(a.keys, rw.grid_b, turn);
@@ -248,14 +247,19 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
     const unsigned lds0 = lds_offset(lds), stat0 = lds_offset(stat);
     const int h0 = hk * rw.G;
     const T *qp = (const T *)rw.q + bz * rw.qb + h0 * rw.qh, *gp = (const T *)a.dout + bz * a.gb + h0 * a.gh;
-    const float *sp = a.stat + ((long)bz * rw.Hk * rw.G + h0) * rw.M;
+    const T *op = (const T *)a.o + bz * a.ob + h0 * a.oh;
+    const float *sp = (OWN ? a.lse : a.stat) + ((long)bz * rw.Hk * rw.G + h0) * rw.M;
     const long stats = (long)rw.grid_b * rw.Hk * rw.G * rw.M;
     const unsigned qrb = (unsigned)(rw.qr * sizeof(T)), qhb = (unsigned)(rw.qh * sizeof(T));
     const unsigned grb = (unsigned)(a.gr * sizeof(T)), ghb = (unsigned)(a.gh * sizeof(T));
+    const unsigned orb = (unsigned)(a.orow * sizeof(T)), ohb = (unsigned)(a.oh * sizeof(T));
     const auto fetch = [&](int r0, int stage) {
         const int n0 = rw.by_g(r0), lane = lane_again();
         const u32x4 qd = dma_buffer(qp + (long)n0 * rw.qr, DMA_MOST), gd = dma_buffer(gp + (long)n0 * a.gr, DMA_MOST);
-        const unsigned at0 = lds0 + stage * 2 * TILE_B;
+        u32x4 od;
+        if constexpr (OWN)
+            od = dma_buffer(op + (long)n0 * a.orow, DMA_MOST);
+        const unsigned at0 = lds0 + stage * STAGE_B;
 #pragma unroll(DT > 2 ? 1 : FL::N)
         for (int x = 0; x < FL::N; ++x)
             if (FL::on(x, wave)) {
@@ -265,8 +269,10 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
                 const bool off = r >= end || c == DMA_OUT;
                 dma16(qd, off ? DMA_OUT : (unsigned)(n - n0) * qrb + g * qhb + c, at0 + FL::lds(x, wave));
                 dma16(gd, off ? DMA_OUT : (unsigned)(n - n0) * grb + g * ghb + c, at0 + TILE_B + FL::lds(x, wave));
+                if constexpr (OWN)
+                    dma16(od, off ? DMA_OUT : (unsigned)(n - n0) * orb + g * ohb + c, at0 + 2 * TILE_B + FL::lds(x, wave));
             }
-        if (wave < 2) {  // a row past the end gets zeros, and has zeros for Q and dO: it adds nothing
+        if (wave < (OWN ? 1 : 2)) {  // a row past the end gets zeros, and has zeros for Q and dO: it adds nothing
             const int r = r0 + lane;
             const int n = rw.by_g(r), g = r - n * rw.G;
             const u32x4 sd = dma_buffer(sp + wave * stats + n0, DMA_MOST);
@@ -297,9 +303,35 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
         __syncthreads();
         if (r0 + BR < end)
             fetch(r0 + BR, stage ^ 1);
+        if constexpr (OWN) {  // P threads of consecutive lanes to a row, every P-th chunk each
+            constexpr int P = 256 / BR;
+            const int tid = wave * 64 + lane_again(), row = tid / P, part = tid % P;
+            const char *gt = lds + stage * STAGE_B + TILE_B, *ot = gt + TILE_B;
+            float s = 0.0f;
+#pragma unroll
+            for (int c = part; c < TL::LC; c += P) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(gt + row * TL::ROWB + 16 * c), y = *reinterpret_cast<const u32x4 *>(ot + row * TL::ROWB + 16 * c);
+                typedef T vec __attribute__((ext_vector_type(TL::EPC)));
+                const vec g = __builtin_bit_cast(vec, x), o = __builtin_bit_cast(vec, y);
+#pragma unroll
+                for (int j = 0; j < TL::EPC; ++j)
+                    s += (float)g[j] * (float)o[j];
+            }
+#pragma unroll
+            for (int k = P / 2; k; k >>= 1)
+                s += __shfl_xor(s, k);
+            if (part == 0) {
+                const float lse = stat[stage * 2 * 64 + row];
+                const bool none = lse == NEG_INF;  // (a row past the end: 0, with zeros for Q and dO)
+                own[row] = none ? POS_INF : lse * 1.44269504088896f;
+                own[64 + row] = none ? 0.0f : s;
+            }
+            __syncthreads();
+        }
+        const float *sl = OWN ? own : stat + stage * 2 * 64, *sd = sl + 64;
 #pragma unroll 1
         for (int s = 0; s < BR / 32; ++s) {
-            const int lane = lane_again(), half = lane >> 5, at0 = stage * 2 * TILE_B + s * 32 * TL::ROWB;
+            const int lane = lane_again(), half = lane >> 5, at0 = stage * STAGE_B + s * 32 * TL::ROWB;
             const int rbase = TL::row_base(lane) + at0, cbase = TL::col_base(lane) + at0;
             const char *qt = lds, *gt = lds + TILE_B;
             f32x16 p, dp;
@@ -311,10 +343,11 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
                 p = mma(TL::row_frag(qt, rbase, 0, t), kf[t], p);
                 dp = mma(TL::row_frag(gt, rbase, 0, t), vf[t], dp);
             }
+            __builtin_amdgcn_sched_barrier(0);  // the statistics' registers only from here on
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const f32x4 ls = *reinterpret_cast<const f32x4 *>(&stat[stage][0][32 * s + 8 * x + 4 * half]);
-                const f32x4 ds = *reinterpret_cast<const f32x4 *>(&stat[stage][1][32 * s + 8 * x + 4 * half]);
+                const f32x4 ls = *reinterpret_cast<const f32x4 *>(sl + 32 * s + 8 * x + 4 * half);
+                const f32x4 ds = *reinterpret_cast<const f32x4 *>(sd + 32 * s + 8 * x + 4 * half);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int i = 4 * x + j;
@@ -357,6 +390,44 @@ __global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void atten
     }
     store_column<T, DT>((T *)a.dk + bz * a.dkb + key * a.dkr + hk * a.dkh, dk, rw.D, half, exists, [&](float x) { return x * a.scale; });
     store_column<T, DT>((T *)a.dv + bz * a.dvb + key * a.dvr + hk * a.dvh, dv, rw.D, half, exists, same);
+}
+
+// the kernel's argument (its only one) where it lies
+__device__ __forceinline__ const AttendBwd &args_again()
+{
+    typedef const __attribute__((address_space(4))) AttendBwd *arg;
+    arg p = (arg)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttendBwd *)p;
+}
+template <typename T, int DT, int WM>
+__global__ __launch_bounds__(256, (attend_dq_per_cu(sizeof(T), DT, WM))) void attend_dq_kernel(AttendBwd a)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[attend_dq_lds(sizeof(T), DT, WM)];
+    __shared__ __attribute__((aligned(16))) float bias[2 * attend_dq_bn(WM)];
+    attend_dq_block<T, DT, WM>(a, lds, bias, blockIdx.x, gridDim.x);
+}
+template <typename T, int DT>
+__global__ __launch_bounds__(256, (attend_dkv_per_cu(sizeof(T), DT))) void attend_dkv_kernel(AttendBwd a)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[attend_dkv_lds(sizeof(T), DT, false)];
+    __shared__ __attribute__((aligned(1024))) float stat[4 * 64];
+    attend_dkv_block<T, DT, false>(a, lds, stat, blockIdx.x, gridDim.x);
+}
+// Both in one launch: where neither fills the card by itself.
+template <typename T, int DT, int WM>
+__global__ __launch_bounds__(256, (attend_both_per_cu(sizeof(T), DT, WM))) void attend_both_kernel(AttendBwd a)
+{
+    constexpr int A = attend_dq_lds(sizeof(T), DT, WM), B = attend_dkv_lds(sizeof(T), DT, true);
+    __shared__ __attribute__((aligned(1024))) char lds[A > B ? A : B];
+    __shared__ __attribute__((aligned(1024))) float small[6 * 64];
+    static_assert(2 * attend_dq_bn(WM) <= 6 * 64, "bias and statistics share their place");
+    // Each side reads the arguments for itself: what both need, loaded once in front of the branch, would not fit the scalar registers.
+    const unsigned n = a.ktiles * a.k_splits * a.rows.Hk * a.rows.grid_b;
+    if (blockIdx.x < n)
+        attend_dkv_block<T, DT, true>(args_again(), lds, small, blockIdx.x, n);
+    else
+        attend_dq_block<T, DT, WM>(args_again(), lds, small, blockIdx.x - n, gridDim.x - n);
 }
 
 // out[row] = f sum_s p[s][row], in slot order; rows of D values, four per lane.  Row -> (batch, n, head) by the strides.  Up to
@@ -410,23 +481,30 @@ __global__ __launch_bounds__(256) void attend_sum_kernel(AttendSums all)
     *reinterpret_cast<x4<T> *>((T *)a.out + b * a.ob + i * a.orow + h * a.oh + d) = v;
 }
 
+template <typename T, int DT, int WM>
+void launch_bwd_shape(const AttendBwd &a, hipStream_t st)
+{
+    const unsigned nq = (unsigned)(a.mtiles * a.q_splits * a.rows.Hk * a.rows.grid_b), nk = (unsigned)(a.ktiles * a.k_splits * a.rows.Hk * a.rows.grid_b);
+    if (a.fused) {
+        hipLaunchKernelGGL((attend_both_kernel<T, DT, WM>), dim3(nq + nk), dim3(256), 0, st, a);
+        return;
+    }
+    if (a.rows.R > 0)
+        hipLaunchKernelGGL((attend_dq_kernel<T, DT, WM>), dim3(nq), dim3(256), 0, st, a);
+    if (a.keys.n > 0)
+        hipLaunchKernelGGL((attend_dkv_kernel<T, DT>), dim3(nk), dim3(256), 0, st, a);
+}
 template <typename T, int DT>
 void launch_bwd_dim(const AttendBwd &a, hipStream_t st)
 {
-    const dim3 block(256);
-    if (a.rows.R > 0) {
-        const dim3 grid((unsigned)(a.mtiles * a.q_splits * a.rows.Hk * a.rows.grid_b));
-        switch (a.wm) {
-        case 1:
-            if constexpr (attend_least_wm(sizeof(T), DT) == 1)
-                hipLaunchKernelGGL((attend_dq_kernel<T, DT, 1>), grid, block, 0, st, a);
-            break;
-        case 2: hipLaunchKernelGGL((attend_dq_kernel<T, DT, 2>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((attend_dq_kernel<T, DT, 4>), grid, block, 0, st, a); break;
-        }
+    switch (a.wm) {
+    case 1:
+        if constexpr (attend_least_wm(sizeof(T), DT) == 1)
+            launch_bwd_shape<T, DT, 1>(a, st);
+        break;
+    case 2: launch_bwd_shape<T, DT, 2>(a, st); break;
+    default: launch_bwd_shape<T, DT, 4>(a, st); break;
     }
-    if (a.keys.n > 0)
-        hipLaunchKernelGGL((attend_dkv_kernel<T, DT>), dim3((unsigned)(a.ktiles * a.k_splits * a.rows.Hk * a.rows.grid_b)), block, 0, st, a);
 }
 
 }  // namespace attend

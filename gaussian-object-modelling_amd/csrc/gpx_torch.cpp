@@ -166,7 +166,7 @@ std::tuple<Tensor, Tensor, Tensor> attend_backward(const Tensor &d_o, const Tens
     a.q = c.in(q, "q", q.sizes(), c.group);
     a.k = c.in(k, "k", ks);
     a.v = c.in(v, "v", ks);
-    a.o = c.in(o, "o", q.sizes());
+    a.o = c.in(o, "o", q.sizes(), c.group);
     a.d_o = c.in(d_o, "d_o", q.sizes(), c.group);
     if (lse.scalar_type() != at::kFloat || lse.device() != q.device() || !lse.is_contiguous())
         refuse("lse must be a contiguous float32 tensor on the device of q");

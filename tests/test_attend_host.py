@@ -110,7 +110,8 @@ def test_workspace_sizes(gpx, at):
 
     assert need(at.FORWARD, batch=8, nq=4096, nk=4096) == 0  # enough workgroups without cutting the keys
     assert need(at.FORWARD, batch=1, nq=1, nk=65536) > 0
-    assert need(at.BACKWARD) >= 2 * 4 * 3 * 8
+    assert need(at.BACKWARD, batch=16, nq=4096, nk=4096) >= 16 * 4 * 4096 * 8  # two floats a row from one launch to the next
+    assert need(at.BACKWARD) == 0  # one launch, nothing cut
     assert need(at.SHARED, n_own=4) > 0
     assert need(at.FORWARD, batch=0) == 0 and need(at.FORWARD, nq=0) == 0 and need(at.FORWARD, nk=0) == 0
 

@@ -134,10 +134,12 @@ def test_many_heads(at, t, shape, kind):
         hold(name, got[name], *want[name])
 
 
+@pytest.mark.parametrize("h,d", [(4, 32), (8, 32), (8, 64)])
 @pytest.mark.parametrize("t", list(TYPES))
-def test_ragged_batch_of_many_workgroups(at, t):
-    """More workgroups than run at once: the batch entries are taken in the order of their lengths (ties, zeros and all)."""
-    b, nq, nk, hq, hk, d = 24, 1100, 150, 4, 4, 32
+def test_ragged_batch_of_many_workgroups(at, t, h, d):
+    """More workgroups than run at once: the batch entries are taken in the order of their lengths (ties, zeros and all), the
+    gradients are two launches."""
+    b, nq, nk, hq, hk = 24, 1100, 150, h, h
     q, k, v, do = inputs(t, b, nq, nk, hq, hk, d, 13)
     n = torch.randint(0, nk + 1, (b,), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
     n[3] = n[4] = n[11] = 77
