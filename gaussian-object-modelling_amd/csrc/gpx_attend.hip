@@ -183,7 +183,7 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
         p.mtiles = (int)blocks_of(R, 32 * wm), p.own_mtiles = (int)blocks_of(Ro, 32 * wo);
         if (a.nk > 0)
             // a piece writes 4 bytes a row and feature where its keys are 2 esz: pieces of wm steps keep that below what they read
-            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), wm, cus, attend_fwd_per_cu(esz, dt, wm, true), &p.splits, &p.chunk);
+            cut(p.mtiles * a.heads_kv, a.nk, attend_fwd_bn(esz, dt, wm), wm, cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
         else
             p.splits = 0;
         if (a.n_own > 0 || a.nk == 0)
@@ -199,7 +199,7 @@ Plan plan_of(const gpx_attend_args &a, int which, int cus)
     p.mtiles = (int)blocks_of(R, 32 * wm);
     const int64_t blocks = p.mtiles * a.heads_kv * a.batch;
     if (which == GPX_ATTEND_FORWARD) {
-        cut(blocks, a.nk, attend_fwd_bn(esz, dt, wm), least_steps(wm), cus, attend_fwd_per_cu(esz, dt, wm, false), &p.splits, &p.chunk);
+        cut(blocks, a.nk, attend_fwd_bn(esz, dt, wm), least_steps(wm), cus, attend_fwd_per_cu(esz, dt, wm), &p.splits, &p.chunk);
         if (p.splits > 1) {
             p.po = up(p.splits * rid * sizeof(float2));
             p.total = p.po + p.splits * rid * a.dim * sizeof(float);
@@ -355,7 +355,7 @@ extern "C" int gpx_attend(const gpx_attend_args *args)
     set_grid(f, p.wm, p.mtiles, p.splits, p.chunk);
     f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
     f.lse = a.lse;
-    f.keys.sort = sorts(a, f.blocks(), cu_count(a) * attend_fwd_per_cu(elem_size(a), attend_dt((int)a.dim), p.wm, false));
+    f.keys.sort = sorts(a, f.blocks(), cu_count(a) * attend_fwd_per_cu(elem_size(a), attend_dt((int)a.dim), p.wm));
     f.slot_rows = (long)(a.batch * a.nq * a.heads);
     if (p.splits > 1) {
         f.pml = (float2 *)((char *)a.workspace + p.ml);

@@ -128,7 +128,7 @@ constexpr int attend_fwd_bn(int esz, int dt, int wm) { return attend_fwd_kt(esz,
 constexpr int attend_fwd_lds(int esz, int dt, int wm, int stages) { return stages * 2 * attend_fwd_bn(esz, dt, wm) * attend_row_bytes(esz, dt); }
 constexpr int attend_lds_per_cu(int bytes) { return bytes <= 38 * 1024 ? 4 : bytes <= 52 * 1024 ? 3 : bytes <= 78 * 1024 ? 2 : 1; }
 // workgroups a CU holds: LDS, and the registers of a wave (512 a SIMD lane, so waves per SIMD = workgroups per CU)
-constexpr int attend_fwd_per_cu(int esz, int dt, int wm, bool pair)
+constexpr int attend_fwd_per_cu(int esz, int dt, int wm)
 {
     const int regs = esz == 4 ? (dt == 1 ? 3 : dt <= 3 ? 2 : 1) : dt <= 2 ? 3 : 2;
     const int lds = attend_lds_per_cu(attend_fwd_lds(esz, dt, wm, 2));

@@ -276,7 +276,7 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
 }
 
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, false))) void attend_fwd_kernel(AttendFwd a)
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_fwd_kernel(AttendFwd a)
 {
     __shared__ __attribute__((aligned(1024))) char lds[attend_fwd_lds(sizeof(T), DT, WM, 2)];
     __shared__ __attribute__((aligned(16))) float bias[2 * attend_fwd_bn(sizeof(T), DT, WM)];
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, false)))
 template <typename T, int DT>
 constexpr int own_wm() { return attend_least_wm(sizeof(T), DT); }
 template <typename T, int DT, int WM>
-__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM, true))) void attend_pair_kernel(AttendPair a)
+__global__ __launch_bounds__(256, (attend_fwd_per_cu(sizeof(T), DT, WM))) void attend_pair_kernel(AttendPair a)
 {
     constexpr int OWN = own_wm<T, DT>();
     constexpr int A = attend_fwd_lds(sizeof(T), DT, WM, 2), B = attend_fwd_lds(sizeof(T), DT, OWN, 1);

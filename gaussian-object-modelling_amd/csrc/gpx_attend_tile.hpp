@@ -143,7 +143,6 @@ struct Tile {
     {
         return LC >= 16 ? (((r & 3) << 2) | ((r >> 2) & 3)) : LC == 8 ? ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : ((r >> 2) & 3);
     }
-    static __device__ __forceinline__ int place(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
 
     // lane part of row_frag's address: row lane % 32, the lane's half of the 16 features of a step
     static __device__ __forceinline__ int row_base(int lane)

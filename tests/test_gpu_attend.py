@@ -385,6 +385,19 @@ def test_streams_and_repeatability(at, t):
             assert torch.equal(a, c)
 
 
+def test_tensors_on_another_device_than_the_current_one(at):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    x = inputs("bf16", 2, 40, 300, 4, 2, 64, 8)
+    a, c = [y.to("cuda:0") for y in x], [y.to("cuda:1") for y in x]
+    o, lse = at.attend(*a[:3])
+    o1, lse1 = at.attend(*c[:3])
+    assert o1.device.index == 1 and torch.cuda.current_device() == 0
+    assert torch.equal(o.cpu(), o1.cpu()) and torch.equal(lse.cpu(), lse1.cpu())
+    for y, z in zip(at.attend_backward(a[3], *a[:3], o, lse), at.attend_backward(c[3], *c[:3], o1, lse1)):
+        assert torch.equal(y.cpu(), z.cpu())
+
+
 def test_captured_and_replayed(at):
     """Two graphs (a training step, a shared call) replayed in turn on new inputs and lengths, with eager work between."""
     b, nq, nk, no, hq, hk, d = 2, 3, 3000, 50, 4, 2, 64
