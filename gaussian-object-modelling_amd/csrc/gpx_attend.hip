@@ -274,12 +274,14 @@ void set_grid(AttendFwd &f, int wm, int mtiles, int splits, int chunk)
     f.by_splits = DivBy((unsigned)std::max(1, splits));
     f.order = attend_order(mtiles, (long)splits * f.rows.Hk * f.rows.grid_b, f.keys.len || f.rows.len);
 }
-AttendKeys keys_of(const gpx_view &k, const gpx_view &v, int64_t n, const int32_t *len, const uint8_t *mask, int64_t mask_b)
+// The kernels take what is left of a buffer from rows x stride.  The stride of a single row says nothing (a broadcast one is 0): dim
+// stands for it.
+AttendKeys keys_of(const gpx_attend_args &a, const gpx_view &k, const gpx_view &v, int64_t n, const int32_t *len, const uint8_t *mask, int64_t mask_b)
 {
     AttendKeys s;
     s.k = k.p, s.v = v.p;
-    s.kb = k.batch, s.kr = k.row, s.kh = k.head;
-    s.vb = v.batch, s.vr = v.row, s.vh = v.head;
+    s.kb = k.batch, s.kr = n > 1 ? k.row : a.dim, s.kh = k.head;
+    s.vb = v.batch, s.vr = n > 1 ? v.row : a.dim, s.vh = v.head;
     s.n = (int)n;
     s.len = len;
     s.mask = mask;
@@ -350,7 +352,7 @@ extern "C" int gpx_attend(const gpx_attend_args *args)
         return GPX_OK;
     AttendFwd f;
     f.rows = rows_of(a);
-    f.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
+    f.keys = keys_of(a, a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
     f.c = (float)(a.scale * ATTEND_LOG2E);
     set_grid(f, p.wm, p.mtiles, p.splits, p.chunk);
     f.o = a.o.p, f.ob = a.o.batch, f.orow = a.o.row, f.oh = a.o.head;
@@ -391,9 +393,9 @@ extern "C" int gpx_attend_shared(const gpx_attend_args *args)
     w.first.rows = w.second.rows = rows_of(a);
     w.first.rows.R = (int)(a.batch * a.nq) * w.first.rows.G;
     w.first.rows.grid_b = 1;
-    w.first.keys = keys_of(a.k, a.v, a.nk, nullptr, nullptr, 0);
+    w.first.keys = keys_of(a, a.k, a.v, a.nk, nullptr, nullptr, 0);
     set_grid(w.first, p.wm, p.mtiles, p.splits, p.chunk);
-    w.second.keys = keys_of(a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
+    w.second.keys = keys_of(a, a.k_own, a.v_own, a.n_own, a.own_len, nullptr, 0);
     w.second.tail = 1;
     w.second.slot0 = p.splits;
     set_grid(w.second, attend_least_wm(elem_size(a), attend_dt((int)a.dim)), p.own_mtiles, p.own_splits, p.own_chunk);
@@ -418,7 +420,7 @@ extern "C" int gpx_attend_backward(const gpx_attend_args *args)
         return GPX_OK;
     AttendBwd b;
     b.rows = rows_of(a);
-    b.keys = keys_of(a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
+    b.keys = keys_of(a, a.k, a.v, a.nk, a.k_len, a.key_mask, a.key_mask_batch);
     b.c = (float)(a.scale * ATTEND_LOG2E);
     b.scale = (float)a.scale;
     b.o = a.o.p, b.ob = a.o.batch, b.orow = a.o.row, b.oh = a.o.head;

@@ -359,8 +359,9 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * at the same time (other streams, graphs replayed side by side) need workspaces of their own.
  *
  * A gpx_view is a tensor [batch][row][head][dim]: base pointer and element strides of the first three axes, dim contiguous;
- * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim) and are at most 2^22 elements
- * apart, the heads of a group in q, d_o and a backward call's o lie within 2^27; an input's batch and head strides may be zero.  Outputs overlap
+ * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim; the row stride of a
+ * single row may be less) and are at most 2^22 elements apart, the heads of a group in q, d_o and a backward call's o lie within
+ * 2^27; an input's batch and head strides may be zero.  Outputs overlap
  * neither each other, their own rows and heads, nor an input.  At most 2^28 rows (batch x nq x heads, and entries) and
  * 2^24 - 1 pieces of work of 32 rows or more a call.  q, o, d_o, dq:
  * [batch][nq][heads][dim]; k, v, dk, dv: [batch][nk][heads_kv][dim]; heads_kv divides heads, query head h reads key head
