@@ -65,7 +65,7 @@ struct AttendFwd {
     long ob = 0, orow = 0, oh = 0;
     float *lse = nullptr;   // [B][H][M]
     float *po = nullptr;    // else: unnormalised sums [slot][rid][D], rid = ((b M + i) H + h)
-    float2 *pml = nullptr;  // and their maximum (log2 units) and sum of weights [slot][rid]
+    float2 *pml = nullptr;  // what their weights are relative to (log2 units) and the sum of weights [slot][rid]
     int slot0 = 0;
     long slot_rows = 0;
 

@@ -23,12 +23,17 @@ namespace attend {
 //                                    beside 16 matrix instructions) and three rounds of 12-tile workgroups
 //   4 x 65536, 32/8 heads of 128 x 3 156 us, 5.2 TB/s: memory
 // STAGES == 1 has one tile at a time (the own part of a shared call: short ranges, many workgroups a CU).
+// fp16 has normal numbers from 2^-14 to 2^15 only: its weights are rounded as 2^LIFT of what they are relative to m, so that an entry
+// 2^-21 of the row's largest still has all its bits (and one of 2^-31 some): many of them can be most of a long context's sum.  The
+// factor is in m, so sums, joins and lse need no other form, and with the lag of 8 below weights stay at or under 2^15.
+template <typename T> constexpr float WEIGHT_LIFT = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 template <typename T, int DT, int WM, int STAGES>
 __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, float *bias, unsigned id, unsigned total)
 {
     using TL = Tile<T, DT>;
     constexpr int WK = 4 / WM, KT = attend_fwd_kt(sizeof(T), DT, WM), NS = KT / 32, BN = KT * WK;
     using FL = Fill<T, DT, BN>;
+    constexpr float LIFT = WEIGHT_LIFT<T>;
     constexpr int TILE_B = BN * TL::ROWB;  // lds: [stage][keys, values]; bias: [stage][BN], 0 or -inf where the key does not count
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -166,11 +171,11 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
             for (int i = 0; i < 16; ++i)
                 top = fmaxf(top, sc[s][i]);
         top = max_both_halves(top) * a.c;
-        // The running maximum need not be the true one: sums in 32 bits and weights of up to 2^8 lose nothing, so it is
-        // raised (and what is summed so far rescaled) only when the new one is more than 8 above it.  (A row without a key
-        // so far has m = -inf, and is raised by any.)
-        if (__any(top > m + 8.0f)) {
-            const float mn = fmaxf(m, top);
+        // The running maximum m + LIFT need not be the true one: sums in 32 bits and weights of up to 2^8 (times 2^LIFT) lose
+        // nothing, so it is raised (and what is summed so far rescaled) only when the new one is more than 8 above it.  (A row
+        // without a key so far has m = -inf, and is raised by any.)
+        if (__any(top > m + (8.0f + LIFT))) {
+            const float mn = fmaxf(m, top - LIFT);
             const float f = mn == NEG_INF ? 1.0f : exp2_(m - mn);
             m = mn;
             l *= f;

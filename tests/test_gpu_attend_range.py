@@ -1,7 +1,12 @@
-"""gpx_attend* at the ends of what the calls take: one entry of any row stride."""
+"""gpx_attend* at the ends of what the calls take: one entry of any row stride, weights far below the largest of their row.  Bounds:
+tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
+import math
 
 import pytest
+
+import attend_oracle as ora
+from attend_oracle import E, F
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -17,6 +22,14 @@ def at(gpu):
 def rnd(t, *shape, seed=0, std=1.0):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(TYPES[t])
 
+
+def hold(name, got, want, bound):
+    got = got.double().cpu()
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]), name
+    off = ((got - want).abs() / bound)[~inf]
+    assert not torch.isnan(off).any(), name
+    assert float(off.max()) <= 1.0, "%s: %.3g of what rounding explains" % (name, float(off.max()))
 
 
 # ---- one entry ---------------------------------------------------------------------------------------------------------------
@@ -58,3 +71,69 @@ def test_one_entry_of_any_row_stride_shared(at, t):
         for args in ((k[0], v[0], own, own), (ctx, ctx, k, v), (k[1], v[1], k, v)):
             x, y = at.attend_shared(q, *args), at.attend_shared(q, *[a.contiguous() for a in args])
             assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+# ---- weights far below the largest ---------------------------------------------------------------------------------------------
+
+def tight(t, q, k, v, scale):
+    """One head (fp64 q [n, d], k, v [m, d]): {name: (value, bound)}.  As attend_oracle's forward, with this absolute term in GPX_F16,
+    which rounds below 2^-14 to multiples of 2^-24 (off by 2^-25): a weight is rounded as 2^7 times its ratio to a reference at
+    most the row's largest, so off by 2^-32 of the row's sum.  Outputs keep the type's own 2^-25."""
+    y = torch.finfo(TYPES[t]).eps / 2
+    u, f16 = (0.0 if t == "f32" else y), t == "f16"
+    out = 2.0 ** -25 if f16 else F
+    (n, d), m = q.shape, k.shape[0]
+    o, lse, _, bl, p, ew = ora.forward(q, k, v, scale, torch.ones(n, m, dtype=torch.bool), TYPES[t])
+    bo = y * o.abs() + (1.01 * u + ew + m * E)[:, None] * (p @ v.abs()) + (2.0 ** -32 if f16 else F) * v.abs().sum(0) + out + m * F
+    return dict(o=(o, bo), lse=(lse, bl))
+
+
+def two_levels(t, n, m, d, below, seed):
+    """Every 32nd entry leads, the others' weights are 2^-below of theirs, and the leaders' values are zero: the result is the tail's."""
+    q, k, v = (rnd(t, x, d, seed=seed + i, std=s) for i, (x, s) in enumerate(((n, 0.05), (m, 0.05), (m, 1.0))))
+    lead = torch.arange(m) % 32 == 0
+    q[:, 0] = 1
+    k[:, 0] = torch.where(lead, 0.0, -below * math.log(2)).to(k.dtype)
+    v = (1000 + 300 * v.float()).to(v.dtype)
+    v[lead] = 0
+    return q, k, v
+
+
+def single(at, t, q, k, v, scale):
+    o, lse = at.attend(*[x.cuda()[None, :, None] for x in (q, k, v)], scale=scale)
+    return dict(o=o[0, :, 0], lse=lse[0, 0])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("below", [10, 14, 17, 20, 22.4, 25.3])
+@pytest.mark.parametrize("n,m,d", [(1, 300, 64), (40, 999, 32), (200, 700, 96), (3, 20000, 128)])
+def test_tail_far_below_the_leaders(at, t, below, n, m, d):
+    q, k, v = two_levels(t, n, m, d, below, 40)
+    want = tight(t, q.double(), k.double(), v.double(), 1.0)
+    got = single(at, t, q, k, v, 1.0)
+    for name in ("o", "lse"):
+        hold(name, got[name], *want[name])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_tail_far_below_the_leaders_shared(at, t):
+    for n, m, own in ((2, 900, 70), (1, 5000, 500)):
+        q, k, v = two_levels(t, n, m + own, 64, 20, 50)
+        want = tight(t, q[-1:].double(), k.double(), v.double(), 1.0)
+        o, lse = at.attend_shared(q.cuda()[None, :, None], k[:m, None].cuda(), v[:m, None].cuda(), k[None, m:, None].cuda(), v[None, m:, None].cuda(),
+                                  scale=1.0)
+        hold("o", o[0, -1:, 0], *want["o"])
+        hold("lse", lse[0, 0, -1:], *want["lse"])
+
+
+def test_long_tail_behind_one_leading_entry(at):
+    """131071 entries 20.9 powers of two below the first one, in rows enough that nothing cuts the range."""
+    n, m, d = 65536, 131072, 64
+    q, k, v = two_levels("f16", 1, m, d, 20.9, 45)
+    v[32::32], k[32::32] = v[31::32][:-1], k[31::32][:-1]
+    want = tight("f16", q.double(), k.double(), v.double(), 1.0)
+    got = single(at, "f16", q.expand(n, d), k, v, 1.0)
+    for name in ("o", "lse"):
+        for row in (0, 777, n - 1):
+            hold(name, got[name][row:row + 1], *want[name])
+        assert bool((got[name] == got[name][:1]).all())
