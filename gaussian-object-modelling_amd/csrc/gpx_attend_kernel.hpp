@@ -186,13 +186,17 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
                     o[d][i] *= f;
         }
         const float sub = EDGE && m == NEG_INF ? 0.0f : m;
+        // The tile's weights are added up before they join l: one at a time, weights 2^-25 of l and less would leave it as it is,
+        // however many there are.
+        float add = 0.0f;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 sc[s][i] = exp2_(sc[s][i] * a.c - sub);
-                l += sc[s][i];
+                add = s == 0 && i == 0 ? sc[s][i] : add + sc[s][i];
             }
+        l += add;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll

@@ -137,3 +137,19 @@ def test_long_tail_behind_one_leading_entry(at):
         for row in (0, 777, n - 1):
             hold(name, got[name][row:row + 1], *want[name])
         assert bool((got[name] == got[name][:1]).all())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_sum_of_very_many_small_weights(at, t):
+    """One leading entry and 2^19 - 1 of 2^-25 of its weight, in rows enough that nothing cuts the range: the sum adds a step's
+    weights up before they join it (32 a lane at most), so that (m / 32 + 40) roundings of 2^-24 stand against 2^19 of them."""
+    n, m, d = 65536, 2 ** 19, 32
+    q = torch.zeros(1, n, 1, d, device="cuda", dtype=TYPES[t])
+    k = torch.zeros(1, m, 1, d, device="cuda", dtype=TYPES[t])
+    q[..., 0] = 1
+    k[:, 1:, :, 0] = -25.0
+    scale = math.log(2)
+    o, lse = at.attend(q, k, torch.zeros_like(k), scale=scale)
+    want = math.log1p((m - 1) * 2.0 ** -25)
+    assert (lse.double() - want).abs().max() <= (m / 32 + 40) * E + 1e-6
+    assert not o.any()
