@@ -17,6 +17,39 @@
 namespace gpx {
 namespace attend {
 
+// fp16 has normal numbers from 2^-14 to 2^15 only, and dS = p (dP - D) may lie anywhere: p as small as 1 / keys, dO of any size (loss
+// scaling).  Each row (dQ) or entry (dK) carries a power of two f: f dS is what is rounded and summed, 1 / f goes over the
+// sum at the end.  f starts far too large and only falls: where the largest |f dS| of a tile passes 2^15 it is brought to 2^7 .. 2^8,
+// what is summed so far with it, and 2^8 of growth are left.  So a dS down to 2^-21 of its row's (entry's) largest so far has all
+// its bits, and none overflows.  The weights for dV are at most 1 and are rounded as 2^12 p.
+// bf16 and fp32 (pieces of bf16) have fp32's range and take dS as it is.
+template <typename T> constexpr bool NARROW = std::is_same_v<T, _Float16>;
+template <typename T> constexpr float P_LIFT = NARROW<T> ? 12.0f : 0.0f;  // (0x1p-12f at the end)
+constexpr float F_START = 0x1p60f, F_MOST = 0x1p15f;
+// the factor that brings top, where it is above F_MOST, to 2^7 .. 2^8
+__device__ __forceinline__ float bring_down(float top)
+{
+    return top > F_MOST ? fminf(__builtin_amdgcn_ldexpf(1.0f, 8 - __builtin_amdgcn_frexp_expf(top)), 1.0f) : 1.0f;  // (infinities: 1)
+}
+__device__ __forceinline__ float reciprocal_of_power(float f) { return __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(unsigned, f)); }
+__device__ __forceinline__ float largest(const f32x16 &w)
+{
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        top = fmaxf(top, __builtin_fabsf(w[i]));
+    return max_both_halves(top);
+}
+template <int DT>
+__device__ __forceinline__ void times(f32x16 (&acc)[DT], float g)
+{
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            acc[d][i] *= g;
+}
+
 // dQ: waves and tiles as in the forward kernel.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
 // The first piece of the key range also leaves each row's statistics for the dK, dV kernel, where that runs behind this one.
 template <typename T, int DT, int WM>
@@ -115,7 +148,7 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
         else
             dd = 0.0f;
         if (!a.fused && split == 0 && wk == 0 && half == 0 && at.exists) {
-            a.stat[rid] = lse;
+            a.stat[rid] = lse - P_LIFT<T>;
             a.stat[(long)rw.grid_b * rw.Hk * rw.G * rw.M + rid] = dd;
         }
     }
@@ -126,6 +159,7 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             dq[d][i] = 0.0f;
+    float f = F_START, fdd = dd * F_START;  // (NARROW)
 
     const auto step = [&](int stage, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
@@ -151,7 +185,19 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            sc[i] = exp2_(sc[i] * a.c - lse) * (dp[i] - dd);
+            sc[i] = exp2_(sc[i] * a.c - lse) * (NARROW<T> ? dp[i] * f - fdd : dp[i] - dd);
+        if constexpr (NARROW<T>) {
+            const float top = largest(sc);
+            if (__any(top > F_MOST)) {
+                const float g = bring_down(top);
+                f *= g;
+                fdd *= g;
+                times<DT>(dq, g);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    sc[i] *= g;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const Frag<T> ds = as_operand<T>(sc, t);
@@ -175,6 +221,8 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
     };
     steps(begin, plain, std::false_type());
     steps(plain, end, std::true_type());
+    if constexpr (NARROW<T>)
+        times<DT>(dq, reciprocal_of_power(f));
     if constexpr (WK > 1) {
         constexpr int PIECE = 64 * 16 * DT;
         static_assert((WK - 1) * WM * PIECE * 4 <= 4 * TILE_B, "the join uses the tiles' memory");
@@ -296,6 +344,7 @@ __device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             dk[d][i] = dv[d][i] = 0.0f;
+    float f = F_START;  // (NARROW)
 
     int stage = 0;
     for (int r0 = begin; r0 < end; r0 += BR, stage ^= 1) {
@@ -323,7 +372,7 @@ __device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, 
             if (part == 0) {
                 const float lse = stat[stage * 2 * 64 + row];
                 const bool none = lse == NEG_INF;  // (a row past the end: 0, with zeros for Q and dO)
-                own[row] = none ? POS_INF : lse * 1.44269504088896f;
+                own[row] = none ? POS_INF : lse * 1.44269504088896f - P_LIFT<T>;
                 own[64 + row] = none ? 0.0f : s;
             }
             __syncthreads();
@@ -362,6 +411,17 @@ __device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, 
                 for (int d = 0; d < DT; ++d)
                     dv[d] = mma(TL::col_frag(gt, cbase, 16 * t, d), w, dv[d]);
             }
+            if constexpr (NARROW<T>) {
+                const float top = largest(dp) * f;
+                if (__any(top > F_MOST)) {
+                    const float g = bring_down(top);
+                    f *= g;
+                    times<DT>(dk, g);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    dp[i] *= f;
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const Frag<T> w = as_operand<T>(dp, t);
@@ -373,6 +433,10 @@ __device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, 
     }
     const int lane = lane_again(), half = lane >> 5, key = key0 + (lane & 31);
     const bool exists = key < a.keys.n, counts = exists && counts_of(key);
+    if constexpr (NARROW<T>) {
+        times<DT>(dk, reciprocal_of_power(f) * 0x1p-12f);
+        times<DT>(dv, 0x1p-12f);
+    }
     // a key that does not count had zeros for its features: its sums are of finite weights but not zero
 #pragma unroll
     for (int d = 0; d < DT; ++d)

@@ -1,4 +1,5 @@
-"""gpx_attend* at the ends of what the calls take: one entry of any row stride, weights far below the largest of their row.  Bounds:
+"""gpx_attend* at the ends of what the calls take: one entry of any row stride, weights and dS far below the largest of their row, d_o
+of any size.  Bounds:
 tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
@@ -75,17 +76,32 @@ def test_one_entry_of_any_row_stride_shared(at, t):
 
 # ---- weights far below the largest ---------------------------------------------------------------------------------------------
 
-def tight(t, q, k, v, scale):
-    """One head (fp64 q [n, d], k, v [m, d]): {name: (value, bound)}.  As attend_oracle's forward, with this absolute term in GPX_F16,
-    which rounds below 2^-14 to multiples of 2^-24 (off by 2^-25): a weight is rounded as 2^7 times its ratio to a reference at
-    most the row's largest, so off by 2^-32 of the row's sum.  Outputs keep the type's own 2^-25."""
+def tight(t, q, k, v, scale, do=None):
+    """One head (fp64 q [n, d], k, v [m, d]): {name: (value, bound)}.  As attend_oracle's forward and backward, with these absolute
+    terms in GPX_F16, which rounds below 2^-14 to multiples of 2^-24 (off by 2^-25): a weight is rounded as 2^7 times its ratio to a
+    reference at most the row's largest, so off by 2^-32 of the row's sum; a weight p for dV as 2^12 p: off by 2^-37; a dS
+    times a power of two that brings the largest of the row (dQ) or of the entry (dK) to 2^7 and more: off by 2^-32 of that one.  Outputs
+    keep the type's own 2^-25."""
     y = torch.finfo(TYPES[t]).eps / 2
     u, f16 = (0.0 if t == "f32" else y), t == "f16"
     out = 2.0 ** -25 if f16 else F
     (n, d), m = q.shape, k.shape[0]
     o, lse, _, bl, p, ew = ora.forward(q, k, v, scale, torch.ones(n, m, dtype=torch.bool), TYPES[t])
     bo = y * o.abs() + (1.01 * u + ew + m * E)[:, None] * (p @ v.abs()) + (2.0 ** -32 if f16 else F) * v.abs().sum(0) + out + m * F
-    return dict(o=(o, bo), lse=(lse, bl))
+    r = dict(o=(o, bo), lse=(lse, bl))
+    if do is None:
+        return r
+    dp, D = do @ v.T, (do * o).sum(1, keepdim=True)
+    ds = p * (dp - D)
+    ep = (ew + 4 * E * lse.abs())[:, None]
+    edp = (d + 2) * E * (do.abs() @ v.abs().T) + (do.abs() * bo).sum(1, keepdim=True) + 2 * d * E * (do.abs() * o.abs()).sum(1, keepdim=True)
+    eds = (1.01 * u + 2 * ep + 4 * E) * ds.abs() + 1.01 * p * edp + F * (dp.abs() + D.abs() + 1)
+    far = 1.01 * 2.0 ** -32 if f16 else 0.0
+    dv, dq, dk = p.T @ do, scale * (ds @ k), scale * (ds.T @ q)
+    r["dv"] = dv, y * dv.abs() + ((1.01 * u + 2 * ep + n * E) * p).T @ do.abs() + (2.0 ** -37 if f16 else F) * do.abs().sum(0) + out + n * F
+    r["dq"] = dq, y * dq.abs() + scale * ((eds + m * E * ds.abs() + far * ds.abs().amax(1, keepdim=True)) @ k.abs()) + out + m * F
+    r["dk"] = dk, y * dk.abs() + scale * ((eds + n * E * ds.abs() + far * ds.abs().amax(0, keepdim=True)).T @ q.abs()) + out + n * F
+    return r
 
 
 def two_levels(t, n, m, d, below, seed):
@@ -99,9 +115,13 @@ def two_levels(t, n, m, d, below, seed):
     return q, k, v
 
 
-def single(at, t, q, k, v, scale):
-    o, lse = at.attend(*[x.cuda()[None, :, None] for x in (q, k, v)], scale=scale)
-    return dict(o=o[0, :, 0], lse=lse[0, 0])
+def single(at, t, q, k, v, scale, do=None):
+    g = [x.cuda()[None, :, None] for x in (q, k, v)]
+    o, lse = at.attend(*g, scale=scale)
+    got = dict(o=o[0, :, 0], lse=lse[0, 0])
+    if do is not None:
+        got.update((a, x[0, :, 0]) for a, x in zip(("dq", "dk", "dv"), at.attend_backward(do.cuda()[None, :, None], *g, o, lse, scale=scale)))
+    return got
 
 
 @pytest.mark.parametrize("t", list(TYPES))
@@ -153,3 +173,63 @@ def test_sum_of_very_many_small_weights(at, t):
     want = math.log1p((m - 1) * 2.0 ** -25)
     assert (lse.double() - want).abs().max() <= (m / 32 + 40) * E + 1e-6
     assert not o.any()
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("below", [12, 18, 22.4])
+@pytest.mark.parametrize("n,m,d", [(64, 300, 64), (33, 999, 32), (200, 700, 96), (2, 9000, 128), (1500, 40, 128)])
+def test_gradients_of_a_tail(at, t, below, n, m, d):
+    q, k, v = two_levels(t, n, m, d, below, 60)
+    v = (v / 512).to(v.dtype)
+    do = (rnd(t, n, d, seed=70, std=0.25).float() + 1).to(q.dtype)
+    want = tight(t, q.double(), k.double(), v.double(), 1.0, do.double())
+    got = single(at, t, q, k, v, 1.0, do)
+    for name in got:
+        hold(name, got[name], *want[name])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("size", [1e-6, 1e-4, 1e-3, 1.0, 1e3])
+@pytest.mark.parametrize("n,m,d", [(64, 300, 64), (130, 4096, 32), (200, 700, 96), (1024, 257, 128)])
+def test_gradients_for_any_size_of_d_o(at, t, size, n, m, d):
+    """q and k of a size that brings dK and dQ near one, whatever d_o is: large with a small scale, or small with a large one."""
+    grow = 2.0 ** round(math.log2(min(max(size, 2.0 ** -10), 2.0 ** 10)))
+    q, k, v, do = (rnd(t, x, d, seed=80 + i, std=s) for i, (x, s) in enumerate(((n, grow), (m, grow), (m, 1.0), (n, size))))
+    scale = d ** -0.5 / grow / grow
+    # dK, dQ = scale sum dS q: of the order of size / grow.  With q, k grown further apart only one of them is near one
+    for x, y in ((q, k), ((q.float() * grow).to(q.dtype), (k.float() / grow).to(k.dtype)), ((q.float() / grow).to(q.dtype), (k.float() * grow).to(k.dtype))):
+        if not bool(torch.isfinite(x).all() and torch.isfinite(y).all()):
+            continue
+        want = tight(t, x.double(), y.double(), v.double(), scale, do.double())
+        got = single(at, t, x, y, v, scale, do)
+        for name in got:
+            hold(name, got[name], *want[name])
+
+
+def test_gradients_of_large_d_o_in_16_bits(at):
+    """dS of some hundred thousand, where scale dS K, scale dS Q and dV fit GPX_F16."""
+    n, m, d = 70, 4, 64
+    q, k = rnd("f16", n, d, seed=90, std=2e-3), rnd("f16", m, d, seed=91, std=2e-3)
+    v, do = rnd("f16", m, d, seed=92, std=100.0), rnd("f16", n, d, seed=93, std=3e3)
+    want = tight("f16", q.double(), k.double(), v.double(), 1.0, do.double())
+    assert max(float(want[name][0].abs().max()) for name in ("dq", "dk", "dv")) < 60000
+    assert float((do.double() @ (v.double() - v.double().mean(0)).T).abs().max()) / m > 2 * 65504
+    got = single(at, "f16", q, k, v, 1.0, do)
+    for name in got:
+        hold(name, got[name], *want[name])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_gradients_that_grow_along_the_context(at, t):
+    """dS grows by many powers of two from the first entries (zero among them) to the last, and falls the other way round."""
+    n, m, d = 48, 640, 64
+    q, k, v, do = (rnd(t, x, d, seed=100 + i, std=s) for i, (x, s) in enumerate(((n, 0.3), (m, 0.3), (m, 1.0), (n, 1e-3))))
+    up = 2.0 ** torch.linspace(-10, 12, m)[:, None]
+    up[:70] = 0
+    rows = 2.0 ** torch.linspace(-3, 9, n)[:, None]
+    for a, c in ((up, rows), (up.flip(0), rows.flip(0))):
+        w, g = (v.float() * a).to(v.dtype), (do.float() * c).to(do.dtype)
+        want = tight(t, q.double(), k.double(), w.double(), 0.3, g.double())
+        got = single(at, t, q, k, w, 0.3, g)
+        for name in got:
+            hold(name, got[name], *want[name])
