@@ -132,6 +132,7 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
     load_row_frags<T, DT>(gf, (const T *)a.dout + (at.valid ? at.b * a.gb + at.i * a.gr + at.h * a.gh : 0), at.valid, rw.D, lane);
     // lse in log2 units (+inf where the row has no weights, so that every p is 0), and <dO, O>
     float lse = POS_INF, dd = 0.0f;
+    bool weights;  // the row has some: else its gradient is zero, whatever it holds and whatever the entries hold
     {
         Frag<T> of[2 * DT];
         load_row_frags<T, DT>(of, (const T *)a.o + (at.valid ? at.b * a.ob + at.i * a.orow + at.h * a.oh : 0), at.valid, rw.D, lane);
@@ -143,7 +144,8 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
             for (int j = 0; j < 8; ++j)
                 dd += gf[t][j] * of[t][j];
         dd = sum_both_halves(dd);
-        if (from != NEG_INF)
+        weights = from != NEG_INF;
+        if (weights)
             lse = from * 1.44269504088896f;
         else
             dd = 0.0f;
@@ -252,10 +254,11 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
     if (a.pq) {
         const long rid = ((long)at.b * rw.M + at.i) * ((long)rw.Hk * rw.G) + at.h;
         float *p = a.pq + ((long)split * ((long)rw.grid_b * rw.M * rw.Hk * rw.G) + rid) * rw.D;
-        store_column<float, DT>(p, dq, rw.D, half, at.exists, [](float x) { return x; });
+        store_column<float, DT>(p, dq, rw.D, half, at.exists, [=](float x) { return weights ? x : 0.0f; });
         return;
     }
-    store_column<T, DT>((T *)a.dq + at.b * a.dqb + at.i * a.dqr + at.h * a.dqh, dq, rw.D, half, at.exists, [&](float x) { return x * a.scale; });
+    store_column<T, DT>((T *)a.dq + at.b * a.dqb + at.i * a.dqr + at.h * a.dqh, dq, rw.D, half, at.exists,
+                        [&](float x) { return weights ? x * a.scale : 0.0f; });
 }
 
 // dK, dV: two waves per SIMD at 128 features (254 registers; with one wave and 372 registers 1767 us where it now takes 1010).  4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one

@@ -1,5 +1,5 @@
 """gpx_attend* at the ends of what the calls take: one entry of any row stride, weights and dS far below the largest of their row, d_o
-of any size.  Bounds:
+of any size, rows that do not count beside NaN.  Bounds:
 tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
@@ -233,3 +233,33 @@ def test_gradients_that_grow_along_the_context(at, t):
         got = single(at, t, q, k, w, 0.3, g)
         for name in got:
             hold(name, got[name], *want[name])
+
+
+# ---- rows that do not count or see nothing, whatever they hold -------------------------------------------------------------------
+
+def bad_values(x):
+    bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(x.dtype).min], dtype=x.dtype)
+    return bad[torch.arange(x.numel()) % 4].reshape(x.shape)
+
+
+EMPTY = [(3, 5, 300, 4, 2, 64), (3, 70, 97, 4, 4, 128), (3, 2, 5000, 2, 1, 96), (3, 600, 40, 4, 1, 32), (24, 1100, 150, 8, 8, 32), (3, 1, 33, 1, 1, 8)]
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", EMPTY, ids=lambda s: "x".join(map(str, s)))
+def test_rows_that_do_not_count_beside_entries_that_are_not_finite(at, t, shape):
+    """q_len: o, lse and dq of the rows behind it are zeros and -inf also where an entry that counts is NaN or infinite."""
+    b, nq, nk, hq, hk, d = shape
+    q, do = rnd(t, b, nq, hq, d, seed=1), rnd(t, b, nq, hq, d, seed=2)
+    k, v = rnd(t, b, nk, hk, d, seed=3), rnd(t, b, nk, hk, d, seed=4)
+    k[1, nk // 2], v[1, nk // 3] = bad_values(k[1, 0]), bad_values(v[1, 0])
+    n = torch.full((b,), nq, dtype=torch.int32)
+    n[1] = nq // 2
+    g = [x.cuda() for x in (q, k, v, do)]
+    o, lse = at.attend(*g[:3], q_len=n.cuda())
+    dq, _, _ = at.attend_backward(g[3], *g[:3], o, lse, q_len=n.cuda())
+    at_ = nq // 2
+    assert not o[1, at_:].any() and bool((lse[1, :, at_:] == -math.inf).all()) and not dq[1, at_:].any()
+    assert bool(torch.isnan(o[1, :at_]).any()) or at_ == 0
+    for i in (0, 2):
+        assert bool(torch.isfinite(o[i]).all() and torch.isfinite(dq[i]).all())
