@@ -1,5 +1,5 @@
 """gpx_attend* at the ends of what the calls take: one entry of any row stride, weights and dS far below the largest of their row, d_o
-of any size, rows that do not count beside NaN.  Bounds:
+of any size, rows without entries that hold NaN.  Bounds:
 tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
@@ -247,6 +247,32 @@ EMPTY = [(3, 5, 300, 4, 2, 64), (3, 70, 97, 4, 4, 128), (3, 2, 5000, 2, 1, 96), 
 
 @pytest.mark.parametrize("t", list(TYPES))
 @pytest.mark.parametrize("shape", EMPTY, ids=lambda s: "x".join(map(str, s)))
+def test_masked_out_members_hold_anything(at, t, shape):
+    """A member whose mask leaves nothing gives zeros, -inf and zero gradients with NaN and infinities in its q, d_o, k and v, as one of
+    length 0 does; the other members' results are those of a call with plain numbers there."""
+    b, nq, nk, hq, hk, d = shape
+    q, do = rnd(t, b, nq, hq, d, seed=1), rnd(t, b, nq, hq, d, seed=2)
+    k, v = rnd(t, b, nk, hk, d, seed=3), rnd(t, b, nk, hk, d, seed=4)
+    mask = torch.rand(b, nk, generator=torch.Generator().manual_seed(5)) > 0.3
+    mask[0, 0] = mask[2, 0] = True
+    mask[1] = False
+
+    def run(*x):
+        g = [y.cuda() for y in x]
+        o, lse = at.attend(*g[:3], key_mask=mask.cuda())
+        return (o, lse) + at.attend_backward(g[3], *g[:3], o, lse, key_mask=mask.cuda())
+
+    plain = run(q, k, v, do)
+    for x in (q, k, v, do):
+        x[1] = bad_values(x[1])
+    got = run(q, k, v, do)
+    for x, y, name in zip(got, plain, ("o", "lse", "dq", "dk", "dv")):
+        assert torch.equal(x, y), name
+    assert not got[0][1].any() and bool((got[1][1] == -math.inf).all()) and not any(x[1].any() for x in got[2:])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", EMPTY, ids=lambda s: "x".join(map(str, s)))
 def test_rows_that_do_not_count_beside_entries_that_are_not_finite(at, t, shape):
     """q_len: o, lse and dq of the rows behind it are zeros and -inf also where an entry that counts is NaN or infinite."""
     b, nq, nk, hq, hk, d = shape
@@ -263,3 +289,27 @@ def test_rows_that_do_not_count_beside_entries_that_are_not_finite(at, t, shape)
     assert bool(torch.isnan(o[1, :at_]).any()) or at_ == 0
     for i in (0, 2):
         assert bool(torch.isfinite(o[i]).all() and torch.isfinite(dq[i]).all())
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("nq,nk", [(40, 300), (2, 5000), (200, 90)])
+def test_a_row_that_is_not_finite_stays_its_own(at, t, nq, nk):
+    """NaN in one query that sees something: NaN in its row of o, lse and dq, the other rows as without it, with a mask and without."""
+    q, do = rnd(t, 2, nq, 2, 64, seed=1), rnd(t, 2, nq, 2, 64, seed=2)
+    k, v = rnd(t, 2, nk, 2, 64, seed=3), rnd(t, 2, nk, 2, 64, seed=4)
+    mask = torch.rand(2, nk, generator=torch.Generator().manual_seed(5)) > 0.3
+    mask[:, 0] = True
+    row = nq // 2
+    for mk in (None, mask.cuda()):
+        for what in (math.nan, math.inf):
+            bad = q.clone()
+            bad[0, row, 1, 5] = what
+            a = at.attend(q.cuda(), k.cuda(), v.cuda(), key_mask=mk)
+            c = at.attend(bad.cuda(), k.cuda(), v.cuda(), key_mask=mk)
+            dq = at.attend_backward(do.cuda(), bad.cuda(), k.cuda(), v.cuda(), *c, key_mask=mk)[0]
+            ref = at.attend_backward(do.cuda(), q.cuda(), k.cuda(), v.cuda(), *a, key_mask=mk)[0]
+            assert bool(torch.isnan(c[0][0, row, 1]).all()) and bool(torch.isnan(c[1][0, 1, row])) and bool(torch.isnan(dq[0, row, 1]).all())
+            for x, y in ((a[0], c[0]), (ref, dq), (a[1].transpose(1, 2), c[1].transpose(1, 2))):
+                x, y = x.clone(), y.clone()
+                x[0, row, 1] = y[0, row, 1] = 0
+                assert torch.equal(x, y)
