@@ -3,11 +3,13 @@
 // Everything is built from one 32 x 32 matrix step with 16 terms of the sum.  Its operand of a lane is 8 values: row (or column)
 // lane % 32, terms 8 (lane / 32) .. + 7; its result is 16 values: column lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4.
 // 16-bit types: one v_mfma_f32_32x32x16.  fp32: each value is cut into three bf16 pieces of 8 bits, exactly (24 bits in all), and
-// of the nine products of pieces the six that reach 2^-24 of the result are summed in fp32, smallest first: the accuracy of a
-// chain of fp32 products (measured error against 64 bits 0.4-1.0 of the plain fp32 form's) at 6 x 32 cycles a step, where
-// v_mfma_f32_32x32x2_f32 takes 8 x 64: 17 x 5 rows over 16384 entries 72 -> 55 us; 4096 x 8192, 8 heads of 128: 157 TFLOP/s, of 64: 170
-// (the fp32 matrix instructions' peak is 157, the library's fp32 product reaches 153; six products at bf16's rate are 178).
-// Values that are not finite become NaN.
+// six of the nine products of pieces are summed in fp32, smallest first.  The pieces of one side are cut off (every m and l has the
+// sign of its value), those of the other rounded to nearest, so what the three left out add up to -- at most 3 x 2^-24 of the product:
+// 2^-7 2^-17 + 2^-15 2^-8 -- has no sign of its own.  (Both cut off: 2^-21, always towards zero, so that it adds up along the
+// features.  Both rounded: 2^-24, but 24 % slower, for the rounding of what the loops read.)  Measured error against 64 bits 0.4-1.0 of a
+// plain fp32 form's, at 6 x 32 cycles a step where v_mfma_f32_32x32x2_f32 takes 8 x 64: 17 x 5 rows over 16384 entries 72 -> 55 us;
+// 4096 x 8192, 8 heads of 128: 154 TFLOP/s, of 64: 142 (the fp32 matrix instructions' peak is 157, the library's fp32 product reaches
+// 153; six products at bf16's rate are 178).  Values that are not finite become NaN.
 //
 // That freedom is used once more: a result tile W (rows = terms of the NEXT product) goes into it as an operand without
 // leaving its lane -- registers 8 t .. 8 t + 7 are the terms { 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4 } -- and the other
@@ -44,32 +46,54 @@ template <typename T>
 struct Frag {
     x8<T> v;
     __device__ __forceinline__ static Frag of(x8<T> x) { return {x}; }
+    __device__ __forceinline__ static Frag rounded(x8<T> x) { return {x}; }
     __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
 };
 template <>
 struct Frag<float> {
     x8<__bf16> h, m, l;  // the upper, middle and lower 8 bits of each value; their sum is the value
+    // cut off: 0 <= m < 2^-7 and 0 <= l < 2^-15 of the value's size, for what the loops read (11 instructions a pair)
     __device__ __forceinline__ static Frag of(x8<float> x)
     {
         u32x4 h, m, l;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            unsigned a[3], b[3];
-            cut(x[2 * j], a);
-            cut(x[2 * j + 1], b);
-            h[j] = __builtin_amdgcn_perm(b[0], a[0], 0x07060302);  // the upper halves of two values
-            m[j] = __builtin_amdgcn_perm(b[1], a[1], 0x07060302);
-            l[j] = __builtin_amdgcn_perm(b[2], a[2], 0x07060302);
+            float a = x[2 * j], b = x[2 * j + 1];
+            h[j] = uppers(a, b);
+            less(a, b, bits(a), bits(b));
+            m[j] = uppers(a, b);
+            less(a, b, bits(a), bits(b));
+            l[j] = uppers(a, b);
         }
         return {__builtin_bit_cast(x8<__bf16>, h), __builtin_bit_cast(x8<__bf16>, m), __builtin_bit_cast(x8<__bf16>, l)};
     }
-    __device__ __forceinline__ static void cut(float x, unsigned (&p)[3])  // pieces in the upper halves
+    // rounded to nearest: |m| <= 2^-8, |l| <= 2^-17, of either sign, for the other side: rows a wave keeps, weights, dS
+    __device__ __forceinline__ static Frag rounded(x8<float> x)
     {
-        p[0] = __builtin_bit_cast(unsigned, x);
-        const float r = x - __builtin_bit_cast(float, p[0] & 0xffff0000u);
-        p[1] = __builtin_bit_cast(unsigned, r);
-        const float s = r - __builtin_bit_cast(float, p[1] & 0xffff0000u);
-        p[2] = __builtin_bit_cast(unsigned, s);
+        constexpr float MOST = 0x1.fep127f;  // bf16's largest: what is above would round to infinity (the lower pieces hold the rest)
+        u32x4 h, m, l;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a = x[2 * j], b = x[2 * j + 1];
+            h[j] = nearest(__builtin_amdgcn_fmed3f(a, -MOST, MOST), __builtin_amdgcn_fmed3f(b, -MOST, MOST));
+            less(a, b, h[j] << 16, h[j]);
+            m[j] = nearest(a, b);
+            less(a, b, m[j] << 16, m[j]);
+            l[j] = uppers(a, b);
+        }
+        return {__builtin_bit_cast(x8<__bf16>, h), __builtin_bit_cast(x8<__bf16>, m), __builtin_bit_cast(x8<__bf16>, l)};
+    }
+    __device__ __forceinline__ static unsigned bits(float x) { return __builtin_bit_cast(unsigned, x); }
+    __device__ __forceinline__ static unsigned uppers(float a, float b) { return __builtin_amdgcn_perm(bits(b), bits(a), 0x07060302); }
+    __device__ __forceinline__ static unsigned nearest(float a, float b)
+    {
+        typedef __bf16 pair __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, pair{(__bf16)a, (__bf16)b});
+    }
+    __device__ __forceinline__ static void less(float &a, float &b, unsigned pa, unsigned pb)  // the pieces' upper halves
+    {
+        a -= __builtin_bit_cast(float, pa & 0xffff0000u);
+        b -= __builtin_bit_cast(float, pb & 0xffff0000u);
     }
     __device__ __forceinline__ float operator[](int j) const { return ((float)l[j] + (float)m[j]) + (float)h[j]; }
 };
@@ -116,7 +140,7 @@ __device__ __forceinline__ float sum_both_halves(float x)
     return a + b;
 }
 
-// 8 values of a result tile as an operand, rounded to the element type (to nearest even; fp32: kept)
+// 8 values of a result tile as an operand, rounded to the element type (to nearest even; fp32: pieces rounded to nearest)
 template <typename T>
 __device__ __forceinline__ Frag<T> as_operand(const f32x16 &w, int t)
 {
@@ -124,7 +148,7 @@ __device__ __forceinline__ Frag<T> as_operand(const f32x16 &w, int t)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         r[j] = (T)w[8 * t + j];
-    return Frag<T>::of(r);
+    return Frag<T>::rounded(r);
 }
 
 // A tile of rows of DP = 32 DT features in LDS: 16-byte chunks, LC (a power of two) per row, chunk c of row r at place
@@ -237,7 +261,7 @@ __device__ __forceinline__ void load_row_frags(Frag<T> (&f)[2 * DT], const T *p,
             else
                 z = *reinterpret_cast<const x8<T> *>(p + d);
         }
-        f[t] = Frag<T>::of(z);
+        f[t] = Frag<T>::rounded(z);
     }
 }
 

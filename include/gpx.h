@@ -374,7 +374,7 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * weights, and in the backward call dS = p (dP - <dO, O>), are rounded to the element type for the products with the values, the
  * queries and the keys, in GPX_F16 times powers of two that go over the sums at the end: a weight keeps its bits down to 2^-21 of the
  * row's largest (2^-26 for dV), a dS of any size down to 2^-21 of its row's (dQ) or its entry's (dK) largest.  GPX_F32 keeps 24
- * bits of values above 2^-100; non-finite entries that count make NaN of what they enter; outputs are rounded once.  Results do not depend on
+ * bits of values above 2^-100 and its products are off by up to 3 x 2^-24 before they are summed; non-finite entries that count make NaN of what they enter; outputs are rounded once.  Results do not depend on
  * timing (fixed order of every sum, no atomics); they may differ in the last bits between devices of another size. */
 typedef enum { GPX_F32 = 0, GPX_F16 = 1, GPX_BF16 = 2 } gpx_scalar;
 typedef enum { GPX_ATTEND_FORWARD = 0, GPX_ATTEND_BACKWARD = 1, GPX_ATTEND_SHARED = 2 } gpx_attend_call;

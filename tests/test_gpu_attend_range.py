@@ -1,5 +1,5 @@
 """gpx_attend* at the ends of what the calls take: one entry of any row stride, weights and dS far below the largest of their row, d_o
-of any size, rows without entries that hold NaN.  Bounds:
+of any size, rows without entries that hold NaN, the pieces of fp32 values.  Bounds:
 tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
@@ -313,3 +313,53 @@ def test_a_row_that_is_not_finite_stays_its_own(at, t, nq, nk):
                 x, y = x.clone(), y.clone()
                 x[0, row, 1] = y[0, row, 1] = 0
                 assert torch.equal(x, y)
+
+
+# ---- fp32 values in pieces -------------------------------------------------------------------------------------------------------
+
+def test_products_of_fp32_values_are_not_biased(at):
+    """One product a score, read from lse = ln 2 * x y.  In units of 2^-24 of it: the pieces left out 3.01 (cut off on one side, m < 2^-7 and
+    l < 2^-15, rounded on the other, m <= 2^-8 and l <= 2^-17), the addition of the last piece 2 whichever way the matrix core rounds,
+    those before it 2^-6 of that, the product with ln 2 1 and ln 2 itself 0.05.  Long runs of ones on both sides, cut off on both, leave
+    out 7.8, always towards zero."""
+    g = torch.Generator().manual_seed(1)
+    x = 1 + torch.rand(4096, generator=g)
+    x[:512] = torch.tensor([0x3f80ffff], dtype=torch.int32).view(torch.float32)   # long runs of ones in the lower bits
+    x[512:1024] = (torch.randint(0x3f80, 0x3fff, (512,), generator=g, dtype=torch.int32) * 65536 + 0xffff).view(torch.float32)
+    x[1024:1536] = (torch.randint(0x3f80, 0x3fff, (512,), generator=g, dtype=torch.int32) * 65536 + 0x7fff).view(torch.float32)
+    x[1536:2048] = (torch.randint(0x3f80, 0x3fff, (512,), generator=g, dtype=torch.int32) * 65536 + 0x8080).view(torch.float32)
+    y = x[torch.cat([torch.arange(512), 512 + torch.randperm(3584, generator=g)])] * torch.where(torch.rand(4096, generator=g) < 0.5, 1.0, -1.0)
+    q, k = torch.zeros(4096, 1, 1, 8), torch.zeros(4096, 1, 1, 8)
+    q[:, 0, 0, 3], k[:, 0, 0, 3] = x, y
+    _, lse = at.attend(q.cuda(), k.cuda(), torch.zeros_like(k).cuda(), scale=math.log(2))
+    want = math.log(2) * x.double() * y.double()
+    off = (lse[:, 0, 0].double().cpu() - want) / want.abs()
+    assert off.abs().max() <= (3.01 + 2.03 + 1.05) * E
+
+
+def test_values_of_any_size_in_fp32_come_through(at):
+    """Weight one: the pieces of a value add up to it, bit for bit, up to the largest there is."""
+    v = torch.randn(64, 1, 2, 64, generator=torch.Generator().manual_seed(2)) * 2.0 ** torch.arange(-90, 38 * 3, 204 / 64)[:64, None, None, None]
+    v.clamp_(-3e38, 3e38)
+    bits = torch.tensor([0x7f7fffff, 0x7f7f8000, 0x7f7f7fff, 0x7f7f0000, 0x7f7effff, 0x3f80ffff, 0x3fffffff, 0x3f808000, 0x3f818000], dtype=torch.int32)
+    v[0, 0, 0, :9] = bits.view(torch.float32)
+    v[0, 0, 1, :9] = -bits.view(torch.float32)
+    for nk in (1, 40):
+        w = torch.full((64, nk, 2, 64), 1.0)
+        w[:, :1] = v
+        k = torch.zeros_like(w)
+        q = torch.ones(64, 3, 2, 64)
+        k[:, 1:] = -100.0
+        o, _ = at.attend(q.cuda(), k.cuda(), w.cuda(), scale=1.0)
+        assert torch.equal(o.cpu(), v.expand(64, 3, 2, 64))
+
+
+def test_values_in_fp32_that_are_not_finite(at):
+    for what in (math.nan, math.inf, -math.inf):
+        q, k, v = (rnd("f32", 2, n, 2, 32, seed=i) for i, n in enumerate((5, 70, 70)))
+        a = at.attend(q.cuda(), k.cuda(), v.cuda())[0]
+        v[0, 33, 1, 7] = what
+        o = at.attend(q.cuda(), k.cuda(), v.cuda())[0]
+        assert not bool(torch.isfinite(o[0, :, 1, 7]).any())
+        o[0, :, 1, 7] = a[0, :, 1, 7]
+        assert torch.equal(o, a)
