@@ -2,6 +2,8 @@
 // cut, workspace layout, launches.  Kernels: gpx_attend_kernel.hpp (forward), gpx_attend_grad.hpp (gradients).
 //
 // Nothing is kept between calls and nothing is allocated: partial sums live in the caller's workspace.
+#include <limits>
+
 #include "gpx_attend.hpp"
 #include "gpx_model.hpp"
 
@@ -71,6 +73,8 @@ int check_args(const gpx_attend_args *pa, int which)
         return fail(GPX_E_BAD_ARG, "negative size");
     if (!(a.scale > 0.0) || !std::isfinite(a.scale) || !std::isfinite((float)(a.scale * ATTEND_LOG2E)))
         return fail(GPX_E_BAD_ARG, "scale must be positive and finite");
+    if (a.scale < (double)std::numeric_limits<float>::min())  // as a float it would lose bits or be 0, and 0 x -inf of a masked entry is NaN
+        return fail(GPX_E_BAD_ARG, "scale must be at least 2^-126");
     if (a.batch > MOST_ROWS || a.nq > MOST_ROWS || a.nk > MOST_ROWS || a.n_own > MOST_ROWS || a.heads > 65536 ||
         a.batch * a.nq > MOST_ROWS || a.batch * a.nq * a.heads > MOST_ROWS ||
         (a.batch > 0 && (std::max(a.nk, a.n_own) / 32 + 1) * a.heads_kv > MOST_ROWS / a.batch))

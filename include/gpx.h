@@ -387,7 +387,7 @@ typedef struct {
     int32_t device;
     int64_t batch, nq, nk, n_own;
     int64_t heads, heads_kv, dim;
-    double scale; /* positive */
+    double scale; /* 2^-126 .. 2^127 */
     gpx_view q, k, v, o;
     float *lse;
     const int32_t *q_len, *k_len;

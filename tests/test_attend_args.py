@@ -1,0 +1,20 @@
+"""CPU suite of the attention calls: refusals of arguments at their ends (tests/test_attend_host.py has the plain ones)."""
+import ctypes as C
+
+import pytest
+
+from test_attend_host import args, at  # noqa: F401  (at: the fixture)
+
+
+@pytest.mark.parametrize("scale", [5e-324, 1e-300, 1e-50, 1e-46, 1e-39, 2.0 ** -126 * (1 - 2.0 ** -52)])
+def test_scales_that_a_float_does_not_hold(gpx, at, scale):  # noqa: F811
+    for which in range(3):
+        assert at._entry(which)(args(at, scale=scale)) == gpx.E_BAD_ARG
+        assert "scale" in gpx.lib().gpx_last_error().decode()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1e-30, 1.0, 2.0 ** 127])
+def test_scales_that_a_float_holds(gpx, at, scale):  # noqa: F811
+    n = C.c_size_t(0)
+    for which in range(3):
+        assert at._entry(3)(args(at, scale=scale), which, C.byref(n)) == gpx.OK

@@ -363,3 +363,17 @@ def test_values_in_fp32_that_are_not_finite(at):
         assert not bool(torch.isfinite(o[0, :, 1, 7]).any())
         o[0, :, 1, 7] = a[0, :, 1, 7]
         assert torch.equal(o, a)
+
+
+# ---- the smallest scale ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_smallest_scale(at, t):
+    """Equal weights for what counts, none for the rest."""
+    q, k, v = (rnd(t, 2, n, 2, 64, seed=i) for i, n in enumerate((40, 75, 75)))
+    mask = torch.rand(2, 75, generator=torch.Generator().manual_seed(5)) > 0.3
+    mask[:, 0] = True
+    want = ora.attend(q, k, v, 2.0 ** -126, ora.seen_of(2, 40, 75, key_mask=mask))
+    o, lse = at.attend(q.cuda(), k.cuda(), v.cuda(), scale=2.0 ** -126, key_mask=mask.cuda())
+    hold("o", o, *want["o"])
+    hold("lse", lse, *want["lse"])
