@@ -5,6 +5,7 @@
 #include <limits>
 
 #include "gpx_attend.hpp"
+#include "gpx_overlap.hpp"
 #include "gpx_model.hpp"
 
 namespace {
@@ -123,6 +124,21 @@ int check_data(const gpx_attend_args &a, int which)
     if (which == GPX_ATTEND_SHARED && (a.q_len || a.k_len || a.key_mask))
         return fail(GPX_E_BAD_ARG, "gpx_attend_shared takes own_len only");
     return GPX_OK;
+}
+
+// an output's batch entries, rows and heads are written by different workgroups
+int check_outputs(const gpx_attend_args &a, int which)
+{
+    const bool rows = a.batch > 0 && a.nq > 0, keys = a.batch > 0 && a.nk > 0;
+    const auto bad = [&](const gpx_view &v, bool on, int64_t n, int64_t heads) {
+        return on && rows_overlap({v.batch, v.row, v.head}, {a.batch, n, heads}, a.dim) != 0;
+    };
+    const char *name = nullptr;
+    if (which != GPX_ATTEND_BACKWARD)
+        name = bad(a.o, rows, a.nq, a.heads) ? "o" : nullptr;
+    else
+        name = bad(a.dq, rows, a.nq, a.heads) ? "dq" : bad(a.dk, keys, a.nk, a.heads_kv) ? "dk" : bad(a.dv, keys, a.nk, a.heads_kv) ? "dv" : nullptr;
+    return name ? fail(GPX_E_BAD_ARG, std::string(name) + ": the batch entries, rows and heads of an output must not overlap") : GPX_OK;
 }
 
 // `pieces` of [0, n) in whole steps of `step`, of at least `least` steps each: where `blocks` workgroups are less than half
@@ -318,6 +334,8 @@ int begin(const gpx_attend_args *pa, int which, DeviceScope &scope, Plan *plan)
     if (rc != GPX_OK)
         return rc;
     rc = scope.enter(pa->device);
+    if (rc == GPX_OK)
+        rc = check_outputs(*pa, which);
     if (rc != GPX_OK)
         return rc;
     *plan = plan_of(*pa, which, cu_count(*pa));

@@ -362,7 +362,8 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim; the row stride of a
  * single row may be less) and are at most 2^22 elements apart, the heads of a group in q, d_o and a backward call's o lie within
  * 2^27; an input's batch and head strides may be zero.  Outputs overlap
- * neither each other, their own rows and heads, nor an input.  At most 2^28 rows (batch x nq x heads, and entries) and
+ * neither each other nor an input, and their own batch entries, rows and heads do not overlap (refused, like interleaved layouts
+ * that take over 2^20 comparisons to tell).  At most 2^28 rows (batch x nq x heads, and entries) and
  * 2^24 - 1 pieces of work of 32 rows or more a call.  q, o, d_o, dq:
  * [batch][nq][heads][dim]; k, v, dk, dv: [batch][nk][heads_kv][dim]; heads_kv divides heads, query head h reads key head
  * h / (heads / heads_kv).  dim: a multiple of 8 up to 128.  lse: [batch][heads][nq] floats, contiguous: log sum_j exp(score).

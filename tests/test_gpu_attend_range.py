@@ -377,3 +377,27 @@ def test_smallest_scale(at, t):
     o, lse = at.attend(q.cuda(), k.cuda(), v.cuda(), scale=2.0 ** -126, key_mask=mask.cuda())
     hold("o", o, *want["o"])
     hold("lse", lse, *want["lse"])
+
+
+# ---- outputs over themselves -------------------------------------------------------------------------------------------------------
+
+def test_outputs_that_overlap_are_refused(gpu):
+    """On the C entry points (attend.py makes its outputs itself): refused before anything is launched, the layouts around them taken."""
+    from test_attend_host import Abi, args
+    at = Abi(gpu.lib())
+    b, n, h, d = 2, 3, 4, 64
+    t = {x: torch.zeros(1 << 14, dtype=torch.bfloat16, device="cuda") for x in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv", "k_own", "v_own")}
+    lse, work = torch.zeros(b * h * n, device="cuda"), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    own = {x: y.data_ptr() for x, y in t.items()}
+    own.update(lse=lse.data_ptr(), workspace=work.data_ptr(), workspace_bytes=work.numel(), batch=b, nq=n, nk=n, n_own=n, heads=h, heads_kv=h, device=0)
+    own.update(ob=768, dqb=768, dkb=768, dvb=768, stream=torch.cuda.current_stream().cuda_stream)
+    assert at._entry(at.FORWARD)(args(at, **own)) == gpu.OK and at._entry(at.BACKWARD)(args(at, **own)) == gpu.OK
+    assert at._entry(at.SHARED)(args(at, **own)) == gpu.OK
+    bad = [(0, 256, 64), (704, 256, 64), (768, 64, 64), (768, 256, 256), (64, 256, 64)]
+    for which, names in ((at.FORWARD, ("ob", "orow", "oh")), (at.SHARED, ("ob", "orow", "oh")), (at.BACKWARD, ("dqb", "dqr", "dqh")),
+                         (at.BACKWARD, ("dkb", "dkr", "dkh")), (at.BACKWARD, ("dvb", "dvr", "dvh"))):
+        for layout in bad:
+            assert at._entry(which)(args(at, **{**own, **dict(zip(names, layout))})) == gpu.E_BAD_ARG, (which, names, layout)
+        for layout in ((768, 64, 192), (2304, 768, 64), (256, 512, 64)):
+            assert at._entry(which)(args(at, **{**own, **dict(zip(names, layout))})) == gpu.OK, (which, names, layout)
+    torch.cuda.synchronize()
