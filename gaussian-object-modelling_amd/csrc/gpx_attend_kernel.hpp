@@ -200,7 +200,7 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
                 for (int i = 0; i < 16; ++i)
                     o[d][i] *= f;
         }
-        const float sub = EDGE && m == NEG_INF ? 0.0f : m;
+        const float sub = m == NEG_INF ? 0.0f : m;  // (no key that counts so far, or only scores below the fp32 range: weights 0)
         // The tile's weights are added up before they join l: one at a time, weights 2^-25 of l and less would leave it as it is,
         // however many there are.
         float add = 0.0f;

@@ -359,11 +359,10 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * at the same time (other streams, graphs replayed side by side) need workspaces of their own.
  *
  * A gpx_view is a tensor [batch][row][head][dim]: base pointer and element strides of the first three axes, dim contiguous;
- * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim; the row stride of a
- * single row may be less) and are at most 2^22 elements apart, the heads of a group in q, d_o and a backward call's o lie within
- * 2^27; an input's batch and head strides may be zero.  Outputs overlap
- * neither each other nor an input, and their own batch entries, rows and heads do not overlap (refused, like interleaved layouts
- * that take over 2^20 comparisons to tell).  At most 2^28 rows (batch x nq x heads, and entries) and
+ * base and strides are multiples of 16 bytes, not negative; rows do not overlap (row >= dim; the row stride of a single row may be
+ * less) and are at most 2^22 elements apart, the heads of a group in q, d_o and a backward call's o lie within 2^27; an input's
+ * batch and head strides may be zero.  Outputs overlap neither each other nor an input, and their own batch entries, rows and heads
+ * do not overlap (refused, like interleaved layouts that take over 2^20 comparisons to tell).  At most 2^28 rows (batch x nq x heads, and entries) and
  * 2^24 - 1 pieces of work of 32 rows or more a call.  q, o, d_o, dq:
  * [batch][nq][heads][dim]; k, v, dk, dv: [batch][nk][heads_kv][dim]; heads_kv divides heads, query head h reads key head
  * h / (heads / heads_kv).  dim: a multiple of 8 up to 128.  lse: [batch][heads][nq] floats, contiguous: log sum_j exp(score).
@@ -373,10 +372,12 @@ int gpx_dgp_optimise(gpx_dgp *g, const gpx_rprop *desc, gpx_rprop_result *res);
  * Queries i >= q_len[b] (NULL: nq) do not count: their o and dq are zero, lse -inf, and they add nothing to dk, dv.  A
  * query without any entry that counts has o = 0, lse = -inf and zero gradients.  Scores, sums and statistics are held in 32 bits;
  * weights, and in the backward call dS = p (dP - <dO, O>), are rounded to the element type for the products with the values, the
- * queries and the keys, in GPX_F16 times powers of two that go over the sums at the end: a weight keeps its bits down to 2^-21 of the
- * row's largest (2^-26 for dV), a dS of any size down to 2^-21 of its row's (dQ) or its entry's (dK) largest.  GPX_F32 keeps 24
- * bits of values above 2^-100 and its products are off by up to 3 x 2^-24 before they are summed; non-finite entries that count make NaN of what they enter; outputs are rounded once.  Results do not depend on
- * timing (fixed order of every sum, no atomics); they may differ in the last bits between devices of another size. */
+ * queries and the keys, in GPX_F16 times powers of two that go over the sums at the end: a weight keeps its bits down to 2^-21 of
+ * the row's largest (2^-26 for dV), a dS of any size down to 2^-21 of its row's (dQ) or its entry's (dK) largest.  GPX_F32 keeps
+ * 24 bits of values above 2^-100 and its products are off by up to 3 x 2^-24 before they are summed.  Outputs are rounded once.
+ * Entries that count and are not finite make NaN of what they enter; a score below the fp32 range is a weight of zero, one above it
+ * makes NaN of its row.  Results do not depend on timing (fixed order of every sum, no atomics); they may differ in the last bits
+ * between devices of another size. */
 typedef enum { GPX_F32 = 0, GPX_F16 = 1, GPX_BF16 = 2 } gpx_scalar;
 typedef enum { GPX_ATTEND_FORWARD = 0, GPX_ATTEND_BACKWARD = 1, GPX_ATTEND_SHARED = 2 } gpx_attend_call;
 typedef struct {

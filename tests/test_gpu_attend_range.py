@@ -1,6 +1,6 @@
 """gpx_attend* at the ends of what the calls take: one entry of any row stride, weights and dS far below the largest of their row, d_o
-of any size, rows without entries that hold NaN, the pieces of fp32 values.  Bounds:
-tests/attend_oracle.py, its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
+of any size, rows without entries that hold NaN, the pieces of fp32 values, scores past the fp32 range.  Bounds: tests/attend_oracle.py,
+its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
 
@@ -401,3 +401,30 @@ def test_outputs_that_overlap_are_refused(gpu):
         for layout in ((768, 64, 192), (2304, 768, 64), (256, 512, 64)):
             assert at._entry(which)(args(at, **{**own, **dict(zip(names, layout))})) == gpu.OK, (which, names, layout)
     torch.cuda.synchronize()
+
+
+# ---- scores past the fp32 range ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,first", [(1, 300, 200), (40, 999, 700), (200, 640, 64), (300, 640, 600)])
+def test_entries_whose_score_is_below_every_number(at, t, nq, nk, first):
+    """Weight zero wherever they lie, also where the first steps of the range hold nothing else."""
+    q, v, do = rnd(t, 1, nq, 1, 64, seed=1), rnd(t, 1, nk, 1, 64, seed=2), rnd(t, 1, nq, 1, 64, seed=3)
+    k = rnd(t, 1, nk, 1, 64, seed=4)
+    q[..., 0], k[..., 0] = 2.0 ** 70, 0.0
+    low = k.clone()
+    low[:, :first, :, :] = 0
+    low[:, :first, :, 0] = -2.0 ** 70
+    o, lse = at.attend(q.cuda(), low.cuda(), v.cuda())
+    n = nk - first
+    want = ora.attend(q, k[:, first:], v[:, first:], 0.125, ora.seen_of(1, nq, n), do)
+    # the zeroth feature adds nothing to a score that counts: its size does not enter the bounds
+    free = q.clone()
+    free[..., 0] = 0
+    plain = ora.attend(free, k[:, first:], v[:, first:], 0.125, ora.seen_of(1, nq, n), do)
+    assert torch.allclose(plain["o"][0], want["o"][0])
+    hold("o", o, plain["o"][0], plain["o"][1])
+    hold("lse", lse, plain["lse"][0], plain["lse"][1])
+    dq, dk, dv = at.attend_backward(do.cuda(), q.cuda(), low.cuda(), v.cuda(), o, lse)
+    hold("dv", dv[:, first:], *plain["dv"])
+    assert not dv[:, :first].any() and not dk[:, :first].any()
