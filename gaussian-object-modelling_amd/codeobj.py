@@ -363,14 +363,11 @@ def _reg_set(tok):
     return {(m.group(1), int(m.group(2)))} if m else set()
 
 
-def mfma_hazard_violations(lines):
-    """lines: the disassembly of ONE kernel (codeobj.disassemble).  Returns [(mfma text, offending text, wait states found,
-    wait states required)] for every instruction that touches the destination of an MFMA on SOME path with fewer wait states
-    than the ISA requires (another MFMA accumulating into the same registers is interlocked and not counted)."""
-    import heapq
+def _flow(lines):
+    """The instructions of ONE kernel's listing as (text, mnemonics, operands, successors, wait states of each)."""
     ins = [(int(l.split("//")[1].split(":")[0], 16), l.split("//")[0].strip(), l) for l in lines if "//" in l]
     if not ins:
-        return []
+        return [], [], [], [], []
     first = ins[0][0]
     at = {a: i for i, (a, _, _) in enumerate(ins)}
     n = len(ins)
@@ -393,6 +390,16 @@ def mfma_hazard_violations(lines):
             nxt = tgt if op == "s_branch" else tgt + nxt
         succ.append(nxt)
         ws.append(int(toks[-1][0]) + 1 if op == "s_nop" else 1)
+    return [text for _, text, _ in ins], ops, toks, succ, ws
+
+
+def mfma_hazard_violations(lines):
+    """lines: the disassembly of ONE kernel (codeobj.disassemble).  Returns [(mfma text, offending text, wait states found,
+    wait states required)] for every instruction that touches the destination of an MFMA on SOME path with fewer wait states
+    than the ISA requires (another MFMA accumulating into the same registers is interlocked and not counted)."""
+    import heapq
+    text, ops, toks, succ, ws = _flow(lines)
+    n = len(ops)
     stores = ("ds_write", "ds_store", "global_store", "flat_store", "buffer_store", "scratch_store", "global_atomic", "ds_add",
               "ds_max", "ds_min", "buffer_atomic", "flat_atomic")
     out = []
@@ -431,7 +438,7 @@ def mfma_hazard_violations(lines):
                         touched |= over
                         need = need_valu
             if w < need and touched & dst:
-                out.append((ins[i][1], ins[j][1], w, need))
+                out.append((text[i], text[j], w, need))
                 continue
             if touched & dst and not (op.startswith("v_mfma") or op.startswith("v_smfmac")):
                 # (past the first legal touch of these registers the MFMA has retired as far as they are concerned; keep
@@ -464,6 +471,57 @@ def guard_mfma_result_hazards(lib_path, tmp_dir):
     assert seen >= 50 and pairs >= 12, (seen, pairs)
 
 
+# ---- scalar registers of asm fetches ------------------------------------------------------------------------------------
+def scalar_hazard_violations(lines):
+    """lines: the disassembly of ONE kernel.  A vector-memory instruction that reads a scalar register needs 5 wait states behind a
+    VALU instruction that wrote it.  hipcc pads that for the instructions it sees, not for those of inline asm.  Returns
+    [(writer, reader, wait states found)] over all paths."""
+    import heapq
+    import re
+
+    def scalars(tok):
+        m = re.fullmatch(r"s\[(\d+):(\d+)\]", tok)
+        if m:
+            return set(range(int(m.group(1)), int(m.group(2)) + 1))
+        m = re.fullmatch(r"s(\d+)", tok)
+        return {int(m.group(1))} if m else {"vcc"} if tok == "vcc" else set()
+    text, ops, toks, succ, ws = _flow(lines)
+    out = []
+    for i, op in enumerate(ops):
+        if not op.startswith("v_") or not toks[i]:
+            continue
+        wrote = set().union(*[scalars(t) for t in toks[i][:2 if "_co_" in op or "div_scale" in op else 1]])
+        if not wrote:
+            continue
+        best, heap = {}, [(0, j) for j in succ[i]]
+        while heap:
+            w, j = heapq.heappop(heap)
+            if w >= 5 or best.get(j, 5) <= w:
+                continue
+            best[j] = w
+            if ops[j].startswith(("buffer_", "global_", "flat_", "scratch_")):
+                if wrote & set().union(*[scalars(t.split()[0]) for t in toks[j] if t]):
+                    out.append((text[i], text[j], w))
+                    continue
+            for k in succ[j]:
+                heapq.heappush(heap, (w + ws[j], k))
+    return out
+
+
+def guard_asm_fetches(lib_path, tmp_dir):
+    """The attention kernels fetch their tiles by inline-asm buffer loads (gpx_attend_tile.hpp, dma16 and dma4), whose buffer and offset
+    the compiler forms as it likes: no VALU write of one of their scalar registers may lie within 5 wait states of them."""
+    seen = 0
+    for sym, lines in disassemble(lib_path, tmp_dir, "attend_").items():
+        fetches = sum(1 for l in lines if l.startswith("buffer_load") and " lds" in l)
+        if not fetches:
+            continue
+        seen += 1
+        bad = scalar_hazard_violations(lines)
+        assert not bad, (sym, bad[:6], len(bad))
+    assert seen >= 100, seen
+
+
 def check_library(lib_path):
     """Every guard above on lib_path; raises AssertionError naming the kernel and the offending instructions."""
     import tempfile
@@ -475,3 +533,4 @@ def check_library(lib_path):
         guard_small_split_accumulators(lib_path, td)
         guard_split_contraction_staging(lib_path, td)
         guard_mfma_result_hazards(lib_path, td)
+        guard_asm_fetches(lib_path, td)
