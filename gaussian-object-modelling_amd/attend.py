@@ -8,7 +8,7 @@ Tensors are [batch, row, head, dim] of one type (float32, float16 or bfloat16) o
 key heads divide the query heads.  Strided views are used as they are where gpx_view in include/gpx.h allows it (contiguous dim,
 base and strides multiples of 16 bytes); other layouts are copied first.  Work is enqueued on the current stream of the tensors'
 device.  What a call refuses raises GpxError.  Gradients are explicit calls, as for gpx_dgp_loglik_gradient: nothing here is
-recorded by autograd.
+recorded by autograd, and attend and attend_shared warn where an input requires gradients (not under torch.no_grad()).
 """
 import importlib.machinery
 import importlib.util

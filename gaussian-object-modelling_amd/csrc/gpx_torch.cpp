@@ -36,7 +36,9 @@ std::string shape_of(at::IntArrayRef s)
 }
 
 struct Call {
+    const bool recording = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;  // nothing here is recorded by autograd
+    bool lost = false;        // an input carries derivatives
     gpx_attend_args a{};
     Tensor q;
     int64_t group = 1;
@@ -71,6 +73,7 @@ struct Call {
     // an input's view; a copy of it where the kernels cannot address it (gpx_view in include/gpx.h)
     gpx_view in(const Tensor &x, const char *name, at::IntArrayRef shape, int64_t heads_of_group = 1)
     {
+        lost = lost || x.requires_grad() || (x.unsafeGetTensorImpl()->autograd_meta() && x._fw_grad(0).defined());
         if (x.scalar_type() != q.scalar_type() || x.device() != q.device())
             refuse(std::string(name) + " must be a tensor of the type and device of q");
         if (x.sizes() != shape)
@@ -114,6 +117,16 @@ struct Call {
         a.key_mask = (const uint8_t *)x->data_ptr();
         a.key_mask_batch = x->stride(0);
     }
+    // a loss over the results would miss these inputs' share of its gradient without a word
+    void warn_of_lost_gradients() const
+    {
+        if (recording && lost &&
+            PyErr_WarnEx(PyExc_UserWarning,
+                         "attend: an input requires gradients, but nothing is recorded by autograd: gradients are explicit calls "
+                         "(attend_backward); under torch.no_grad() this warning is not given",
+                         2) < 0)
+            throw py::error_already_set();
+    }
     void run(int which, int (*call)(const gpx_attend_args *), uint64_t stream)
     {
         a.stream = (void *)stream;
@@ -151,6 +164,7 @@ std::tuple<Tensor, Tensor> attend(const Tensor &q, const Tensor &k, const Tensor
     Tensor o = c.out(q.sizes(), a.o);
     Tensor lse = at::empty({a.batch, a.heads, a.nq}, c.like.dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
+    c.warn_of_lost_gradients();
     c.run(GPX_ATTEND_FORWARD, gpx_attend, stream);
     return {o, lse};
 }
@@ -201,6 +215,7 @@ std::tuple<Tensor, Tensor> attend_shared(const Tensor &q, const Tensor &k, const
     Tensor o = c.out(q.sizes(), a.o);
     Tensor lse = at::empty({a.batch, a.heads, a.nq}, c.like.dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
+    c.warn_of_lost_gradients();
     c.run(GPX_ATTEND_SHARED, gpx_attend_shared, stream);
     return {o, lse};
 }

@@ -3,6 +3,7 @@ of any size, rows without entries that hold NaN, the pieces of fp32 values, scor
 its absolute terms for GPX_F16 replaced by what the kernels keep (tight)."""
 import importlib
 import math
+import warnings
 
 import pytest
 
@@ -428,3 +429,28 @@ def test_entries_whose_score_is_below_every_number(at, t, nq, nk, first):
     dq, dk, dv = at.attend_backward(do.cuda(), q.cuda(), low.cuda(), v.cuda(), o, lse)
     hold("dv", dv[:, first:], *plain["dv"])
     assert not dv[:, :first].any() and not dk[:, :first].any()
+
+
+# ---- gradients that nothing records --------------------------------------------------------------------------------------------------
+
+def test_inputs_that_require_gradients_are_warned_of(at):
+    q, k = rnd("f32", 2, 5, 4, 64, seed=1).cuda(), rnd("f32", 2, 9, 4, 64, seed=2).cuda()
+    leaf = k.clone().requires_grad_()
+    calls = [lambda x: at.attend(q, x, k), lambda x: at.attend(q, k, x), lambda x: at.attend_shared(q, x[0], k[0], k, k), lambda x: at.attend_shared(q, k[0], k[0], k, x)]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        ref = [call(k) for call in calls]
+        with torch.no_grad():
+            for call, y in zip(calls, ref):
+                assert torch.equal(call(leaf)[0], y[0])
+        with pytest.raises(UserWarning):
+            calls[0](leaf)
+        at.attend_backward(q, q, leaf, k, *at.attend(q, leaf.detach(), k))
+    for call, y in zip(calls, ref):
+        with pytest.warns(UserWarning, match="attend_backward") as w:
+            o, lse = call(leaf)
+        assert not o.requires_grad and torch.equal(o, y[0]) and torch.equal(lse, y[1])
+        assert w[0].filename == __file__
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.warns(UserWarning):
+            at.attend(torch.autograd.forward_ad.make_dual(q, torch.ones_like(q)), k, k)
