@@ -115,22 +115,7 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
     }
 
     Frag<T> qf[2 * DT];
-    const T *qp = (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0);
-    load_row_frags<T, DT>(qf, qp, at.valid, rw.D, lane);
-    // A masked key starts at -inf and has zeros for features: that holds for a finite query only.  Any other is taken as zeros,
-    // and its sum of weights becomes NaN if it has any.
-    bool bad = false;
-    if (mask) {
-        float z = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2 * DT; ++t)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                z += qf[t][j] * 0.0f;
-        bad = sum_both_halves(z) != 0.0f;
-        if (__any(bad))
-            load_row_frags<T, DT>(qf, qp, at.valid && !bad, rw.D, lane);
-    }
+    load_row_frags<T, DT>(qf, (const T *)rw.q + (at.valid ? at.b * rw.qb + at.i * rw.qr + at.h * rw.qh : 0), at.valid, rw.D, lane);
 
     f32x16 o[DT];
 #pragma unroll
@@ -246,8 +231,15 @@ __device__ __forceinline__ void attend_fwd_block(const AttendFwd &a, char *lds, 
     steps(begin, plain, std::false_type());
     steps(plain, end, std::true_type());
     l = sum_both_halves(l);
-    if (bad && l != 0.0f)
-        l = __builtin_nanf("");
+    // A masked key starts at -inf and has zeros for features, which a query that is not finite turns into NaN: where no key of
+    // this piece counts the row has seen nothing all the same.
+    if (mask && __any(l != l)) {
+        bool some = false;
+        for (int j = begin + lane; j < end; j += 64)
+            some = some || mask[j];
+        if (!__any(some))
+            m = NEG_INF, l = 0.0f;
+    }
 
     if constexpr (WK > 1) {  // join the waves' pieces of the key range, in wave order
         constexpr int PIECE = 64 * 16 * DT + 128;
