@@ -50,12 +50,14 @@ def attend(q, k, v, scale=None, k_len=None, key_mask=None, q_len=None):
 
 
 def attend_backward(d_o, q, k, v, o, lse, scale=None, k_len=None, key_mask=None, q_len=None):
-    """dq, dk, dv for the gradient d_o of attend's o; o and lse as attend returned them, the other arguments as it got them."""
+    """dq, dk, dv for the gradient d_o of attend's o; o and lse as attend returned them, the other arguments as it got them.  d_o may be
+    of any size (loss scaling): in float16 too only results that float16 does not hold are lost."""
     return (_loaded or ext()).attend_backward(d_o, q, k, v, o, lse, scale, k_len, key_mask, q_len, _stream(q))
 
 
 def attend_shared(q, k, v, k_own, v_own, own_len=None, scale=None):
     """o and lse (as attend) of a batch over ONE context: q [batch, nq, heads, dim]; k, v [nk, heads_kv, dim], which every query
     sees; k_own, v_own [batch, n_own, heads_kv, dim], of which own_len[b] (int32 [batch]; None: all) exist, the rows of the nq
-    queries last: query i sees the own entries j < own_len[b] - (nq - 1 - i).  The context is read once for the whole batch."""
+    queries last: query i sees the own entries j < own_len[b] - (nq - 1 - i).  The context is read once for the whole batch.  There
+    is no gradient call for it."""
     return (_loaded or ext()).attend_shared(q, k, v, k_own, v_own, own_len, scale, _stream(q))

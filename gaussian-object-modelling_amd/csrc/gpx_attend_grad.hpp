@@ -6,9 +6,9 @@
 // with the rows held by the wave, dK and dV with the keys held by the wave.  No atomics: every sum has a fixed order.  (One kernel
 // with 5 products would have to add dQ up over the key tiles: in memory, 64 partial sums of it at 8191 keys, or by atomics, whose
 // order changes the result.)
-// bf16, 2 x 4096 queries, 8191 keys, 16 heads of 128: dQ 742 us = 1111 TFLOP/s, dK dV 1010 us = 1088 TFLOP/s -- both at the rate of the
-// library's large products; the 7 products are what is left.  Ragged and small shapes are bound by latency: eight objects with
-// 16 / 4 heads of 64: 43 and 61 us.
+// bf16, 2 x 4096 queries, 8191 keys, 16 heads of 128, from card to card: dQ 736 to 752 us = 1120 to 1096 TFLOP/s, dK dV 1010 to 1061 us =
+// 1088 to 1036 TFLOP/s -- about the rate of the library's large products; the 7 products are what is left.  Ragged and small shapes
+// are bound by latency: eight objects with 16 / 4 heads of 64 in fp16: 47 and 63 us (without the powers of two below: 42 and 60).
 #pragma once
 #include <type_traits>
 
@@ -261,8 +261,9 @@ __device__ __forceinline__ void attend_dq_block(const AttendBwd &a, char *lds, f
                         [&](float x) { return weights ? x * a.scale : 0.0f; });
 }
 
-// dK, dV: two waves per SIMD at 128 features (254 registers; with one wave and 372 registers 1767 us where it now takes 1010).  4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding one
-// key, then dV^T += dO^T P and dK^T += Q^T dS.
+// dK, dV: two waves per SIMD at 128 features of 16 bits (241 registers, fp16 245; one wave with 372 registers took 1767 us where this
+// takes 1010 to 1061).  4 waves of 32 keys each; the rows pass through LDS in tiles of BR.  S = Q K^T and dP = dO V^T with a lane holding
+// one key, then dV^T += dO^T P and dK^T += Q^T dS.
 // OWN: in one launch with dQ; <dO, O> is formed here, from tiles of O beside those of dO, once per tile by all threads.
 template <typename T, int DT, bool OWN>
 __device__ __forceinline__ void attend_dkv_block(const AttendBwd &a, char *lds, float *stat, unsigned id, unsigned total)

@@ -17,10 +17,11 @@ namespace attend {
 // Keys and values are read from memory once per 32 WM rows, as tiles of BN rows, two of them in LDS: while one is worked on the
 // next is on its way.  64 keys a wave and step for the 16-bit types with WM = 4 (32: as fast at 64 and slower at 96 features).
 // What bounds it (bf16; the library's 8192^3 product reaches 1067 TFLOP/s on the same card):
-//   16384 x 16384, 16 heads of 128   2.06 ms, 1066 TFLOP/s: the matrix cores at the card's power limit (clock 1.9-2.1 GHz; without
-//                                    the softmax 2.01, without any fetch 1.95)
-//   32768 x 724, 8 heads of 64       67 us, 727 TFLOP/s: vector issue (153 instructions a tile and wave, 128 of them the softmax's,
-//                                    beside 16 matrix instructions) and three rounds of 12-tile workgroups
+//   16384 x 16384, 16 heads of 128   2.06 to 2.15 ms from card to card, 1066 to 1023 TFLOP/s: the matrix cores at the card's power limit
+//                                    (clock 1.9-2.1 GHz; without the softmax 2.01, without any fetch 1.95)
+//   32768 x 724, 8 heads of 64       67 us, 724 TFLOP/s: neither vector issue (59 % of the SIMDs' time; 156 instructions a tile and wave,
+//                                    128 of them the softmax's) nor matrix cores (31 %) are full: 2048 workgroups of 12 tiles on
+//                                    768 places are 2.7 rounds paid as three, each with its own start and end
 //   4 x 65536, 32/8 heads of 128 x 3 156 us, 5.2 TB/s: memory
 // STAGES == 1 has one tile at a time (the own part of a shared call: short ranges, many workgroups a CU).
 // fp16 has normal numbers from 2^-14 to 2^15 only: its weights are rounded as 2^LIFT of what they are relative to m, so that an entry

@@ -1,6 +1,6 @@
 // gpx_torch.cpp -- torch tensors in front of gpx_attend, gpx_attend_backward and gpx_attend_shared (include/gpx.h); attend.py documents
 // the calls.  Checks, views, output and workspace allocation in C++ because the smallest calls cost little more than that: one
-// query over 277 entries took 12.4 us a call with these steps in Python (a kernel launch is 4.5 of them).  No arithmetic here.
+// query over 277 entries took 12.1 us a call with these steps in Python (a kernel launch is 4.5 of them).  No arithmetic here.
 #include <torch/extension.h>
 
 #include <cmath>
